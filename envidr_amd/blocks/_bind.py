@@ -1,0 +1,76 @@
+"""ctypes signatures of include/envidr_blocks.h and the checks its wrappers share."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _lib
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_P, _U, _U64, _I64, _I, _D = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int64, ctypes.c_int, ctypes.c_double
+
+# entry point -> (result, arguments); include/envidr_blocks.h in its order
+SIGNATURES = {
+    "envidr_blocks_abi_version": (_I, []),
+    "envidr_gated_mlp_workspace_bytes": (_U64, [_U, _U, _U, _U, _I, _I]),
+    "envidr_gated_mlp_forward": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _U, _U, _U, _U, _I, _I, _P, _I64, _P, _U64, _P]),
+    "envidr_gated_mlp_backward": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _U, _U, _U, _U, _I, _I, _P, _I64, _P, _P, _P, _P, _U64, _P]),
+    "envidr_ray_recurrence_saved_floats": (_U64, [_U64, _U, _U]),
+    "envidr_ray_recurrence_workspace_bytes": (_U64, [_U64, _U, _U]),
+    "envidr_ray_recurrence_forward": (_I, [_P, _P, _P, _P, _U64, _U, _U, _I, _I, _P, _P, _P, _P, _U64, _P]),
+    "envidr_ray_recurrence_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _U64, _U, _U, _I, _I, _P, _P, _P, _P, _U64, _P]),
+    "envidr_dropout": (_I, [_P, _P, _P, _U64, _D, _I, _P, _P]),
+    "envidr_dropout_step": (_I, [_P, _P, _P]),
+}
+
+_bound = None
+
+
+def lib() -> ctypes.CDLL:
+    """the library with this header's entry points bound; raises if it lacks one"""
+    global _bound
+    if _bound is None:
+        loaded = _lib.load()
+        for name, (result, arguments) in SIGNATURES.items():
+            fn = getattr(loaded, name, None)
+            if fn is None:
+                raise _lib.EnvidrError(f"libenvidr_amd.so does not export {name}")
+            fn.restype, fn.argtypes = result, arguments
+        _bound = loaded
+    return _bound
+
+
+def check(rc: int, name: str) -> None:
+    if rc:
+        raise _lib.EnvidrError(f"{name} failed ({rc}): {lib().envidr_last_error().decode()}")
+
+
+def same_kind(name: str, first: torch.Tensor, **others: torch.Tensor | None) -> int:
+    """the dtype code of `first`; raises unless it is a GPU tensor of a supported dtype and the others share its dtype and device"""
+    if not first.is_cuda:
+        raise _lib.EnvidrError(f"{name}: needs GPU tensors (got a {first.device} tensor); envidr_amd has no CPU path")
+    if first.dtype not in DTYPES:
+        raise _lib.EnvidrError(f"{name}: {first.dtype} is not one of {', '.join(str(d) for d in DTYPES)}")
+    for what, t in others.items():
+        if t is not None and (t.dtype != first.dtype or t.device != first.device):
+            raise _lib.EnvidrError(f"{name}: {what} is {t.dtype} on {t.device}, the first tensor {first.dtype} on {first.device}")
+    return DTYPES[first.dtype]
+
+
+class on_device:
+    """The tensor's device as the current one for the launches inside (a no-op when it is already), and its current stream."""
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+        self.before = None
+
+    def __enter__(self) -> int:
+        if torch.cuda.current_device() != self.index:
+            self.before = torch.cuda.current_device()
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.before is not None:
+            torch.cuda.set_device(self.before)

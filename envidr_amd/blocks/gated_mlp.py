@@ -1,0 +1,108 @@
+"""The gated feed-forward block (envidr_gated_mlp_*, csrc/gated_mlp.hip):  y = (act(x Wg^T) * (x Wu^T)) Wd^T  and its gradients."""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from . import _bind
+from .dropout import CounterDropout
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}      # gelu: the tanh form
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """a matrix whose rows the kernels can walk: adjacent elements, any row pitch that keeps rows apart"""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) <= 1 << 21 else t.contiguous()
+
+
+def _sizes(x, wg, wd):
+    return x.shape[0], x.shape[1], wg.shape[0], wd.shape[0]
+
+
+def _workspace(lib, M, D, F, O, code, backward, device):
+    n = lib.envidr_gated_mlp_workspace_bytes(M, D, F, O, code, backward)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device), n
+
+
+def _forward(x, wg, wu, wd, code, act):
+    lib = _bind.lib()
+    M, D, F, O = _sizes(x, wg, wd)
+    y = torch.empty(M, O, dtype=x.dtype, device=x.device)
+    with _bind.on_device(x) as stream:
+        ws, n = _workspace(lib, M, D, F, O, code, 0, x.device)
+        _bind.check(lib.envidr_gated_mlp_forward(x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), wd.data_ptr(), wd.stride(0),
+                                                 M, D, F, O, code, act, y.data_ptr(), O, ws.data_ptr(), n, stream), "envidr_gated_mlp_forward")
+    return y
+
+
+class _GatedMlp(torch.autograd.Function):
+    """Keeps x and the weights: the backward pass forms the hidden layer again."""
+
+    @staticmethod
+    def forward(ctx, x, wg, wu, wd, code, act):
+        ctx.save_for_backward(x, wg, wu, wd)
+        ctx.code, ctx.act = code, act
+        return _forward(x, wg, wu, wd, code, act)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, wg, wu, wd = ctx.saved_tensors
+        lib = _bind.lib()
+        M, D, F, O = _sizes(x, wg, wd)
+        dy = _rows(dy)
+        new = lambda want, *shape: torch.empty(*shape, dtype=x.dtype, device=x.device) if want else None  # noqa: E731
+        grads = [new(want, *shape) for want, shape in zip(ctx.needs_input_grad, ((M, D), (F, D), (F, D), (O, F)))]
+        at = [None if g is None else g.data_ptr() for g in grads]
+        with _bind.on_device(x) as stream:
+            ws, n = _workspace(lib, M, D, F, O, ctx.code, 1, x.device)
+            _bind.check(lib.envidr_gated_mlp_backward(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0),
+                                                      wd.data_ptr(), wd.stride(0), M, D, F, O, ctx.code, ctx.act, at[0], D, at[1], at[2], at[3],
+                                                      ws.data_ptr(), n, stream), "envidr_gated_mlp_backward")
+        return (*grads, None, None)
+
+
+def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """(act(x Wg^T) * (x Wu^T)) Wd^T:  x [..., D], w_gate and w_up [F, D], w_down [O, F] (as nn.Linear keeps them) -> [..., O].
+
+    One dtype (float32, bfloat16 or float16) and one device for all; any strides; activation "silu", "gelu" (tanh form), "relu" or
+    "sigmoid".  Differentiable once, w.r.t. every tensor.  Products accumulate in 32 bits; in the 16-bit dtypes the hidden layer is rounded
+    to the dtype once, between the products.  float32 carries 24-bit operands through the bf16 matrix cores; an infinity in them gives NaN."""
+    code = _bind.same_kind("gated_mlp", x, w_gate=w_gate, w_up=w_up, w_down=w_down)
+    if activation not in ACTIVATIONS:
+        raise _lib.EnvidrError(f"gated_mlp: activation {activation!r} is not one of {', '.join(ACTIVATIONS)}")
+    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.dim() != 2 or w_down.shape[1] != w_gate.shape[0] or x.shape[-1] != w_gate.shape[1]:
+        raise _lib.EnvidrError(f"gated_mlp: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}: "
+                               "x [..., D], w_gate and w_up [F, D], w_down [O, F] are wanted")
+    if 0 in w_gate.shape or 0 in w_down.shape:
+        raise _lib.EnvidrError("gated_mlp: a width is zero")
+    rows = _rows(x.reshape(-1, x.shape[-1]))
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+        y = _GatedMlp.apply(rows, _rows(w_gate), _rows(w_up), _rows(w_down), code, ACTIVATIONS[activation])
+    else:
+        y = _forward(rows, _rows(w_gate), _rows(w_up), _rows(w_down), code, ACTIVATIONS[activation])
+    return y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+class GatedMLP(torch.nn.Module):
+    """A gated feed-forward block of width d_in -> d_hidden -> d_out (d_in when not given), without biases.  residual: adds x to the result; p: dropout
+    on the result in training."""
+
+    def __init__(self, d_in: int, d_hidden: int, d_out: int | None = None, activation: str = "silu", residual: bool = False, p: float = 0.0, seed: int = 0):
+        super().__init__()
+        d_out = d_in if d_out is None else d_out
+        if residual and d_out != d_in:
+            raise _lib.EnvidrError(f"GatedMLP: a residual needs d_out = d_in, not {d_out} and {d_in}")
+        if activation not in ACTIVATIONS:
+            raise _lib.EnvidrError(f"GatedMLP: activation {activation!r} is not one of {', '.join(ACTIVATIONS)}")
+        self.activation, self.residual = activation, residual
+        self.w_gate = torch.nn.Parameter(torch.empty(d_hidden, d_in))
+        self.w_up = torch.nn.Parameter(torch.empty(d_hidden, d_in))
+        self.w_down = torch.nn.Parameter(torch.empty(d_out, d_hidden))
+        for w in (self.w_gate, self.w_up, self.w_down):
+            torch.nn.init.xavier_uniform_(w)
+        self.drop = CounterDropout(p, seed)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = gated_mlp(x, self.w_gate, self.w_up, self.w_down, self.activation)
+        return self.drop(y, residual=x if self.residual else None)

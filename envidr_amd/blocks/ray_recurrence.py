@@ -1,0 +1,85 @@
+"""A gated linear recurrence along the samples of packed rays (envidr_ray_recurrence_*, csrc/ray_recurrence.hip)."""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from . import _bind
+
+
+def _workspace(lib, T, N, C, device):
+    n = lib.envidr_ray_recurrence_workspace_bytes(T, N, C)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device), n
+
+
+def _forward(gate, value, rays, state, code, blend, keep):
+    lib = _bind.lib()
+    T, C = gate.shape
+    N = rays.shape[0]
+    h = torch.empty(T, C, dtype=gate.dtype, device=gate.device)
+    # (an id that no ray names keeps its state)
+    last = torch.zeros(N, C, dtype=torch.float32, device=gate.device) if state is None else state.clone()
+    saved = torch.empty(lib.envidr_ray_recurrence_saved_floats(T, N, C), dtype=torch.float32, device=gate.device) if keep else None
+    with _bind.on_device(gate) as stream:
+        ws, n = _workspace(lib, T, N, C, gate.device)
+        _bind.check(lib.envidr_ray_recurrence_forward(gate.data_ptr(), value.data_ptr(), rays.data_ptr(), None if state is None else state.data_ptr(), T, N, C, code, blend,
+                                                      h.data_ptr(), last.data_ptr(), None if saved is None else saved.data_ptr(), ws.data_ptr(), n, stream),
+                    "envidr_ray_recurrence_forward")
+    return h, last, saved
+
+
+class _RayRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, value, state, rays, code, blend):
+        h, last, saved = _forward(gate, value, rays, state, code, blend, True)
+        ctx.save_for_backward(gate, value, state, rays, saved)
+        ctx.code, ctx.blend = code, blend
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast):
+        gate, value, state, rays, saved = ctx.saved_tensors
+        lib = _bind.lib()
+        T, C = gate.shape
+        N = rays.shape[0]
+        dh = dh.contiguous()
+        dlast = dlast.contiguous()
+        dgate, dvalue = torch.empty_like(gate), torch.empty_like(value)
+        dstate = dlast.clone() if ctx.needs_input_grad[2] else None          # (an id that no ray names: last was its state)
+        with _bind.on_device(gate) as stream:
+            ws, n = _workspace(lib, T, N, C, gate.device)
+            _bind.check(lib.envidr_ray_recurrence_backward(dh.data_ptr(), dlast.data_ptr(), gate.data_ptr(), value.data_ptr(), rays.data_ptr(),
+                                                           None if state is None else state.data_ptr(), saved.data_ptr(), T, N, C, ctx.code, ctx.blend,
+                                                           dgate.data_ptr(), dvalue.data_ptr(), None if dstate is None else dstate.data_ptr(), ws.data_ptr(), n, stream),
+                        "envidr_ray_recurrence_backward")
+        return dgate, dvalue, dstate, None, None, None
+
+
+def ray_recurrence(gate: torch.Tensor, value: torch.Tensor, rays: torch.Tensor, state: torch.Tensor | None = None, blend: bool = True):
+    """h_t = a_t h_{t-1} + (1 - a_t) value_t, a_t = sigmoid(gate_t), along the samples of each ray -> (h [T, C], last [N, C]).
+
+    gate, value [T, C] (float32, bfloat16 or float16), rays int32 [N, 3] = (id, offset, count) as `march_rays_train` returns them: rows offset ..
+    offset + count - 1 are one ray's samples in order; rays may come in any order but share no rows.  state float32 [N, C]: h before the
+    first sample, by id (zeros when not given); last float32 [N, C]: h after the last one, to go on from.  blend=False: h_t = a_t h_{t-1} + value_t.
+    Rows that belong to no ray, and their gradients, are zero.  States are carried in 32 bits.  Differentiable once w.r.t. gate, value and state."""
+    code = _bind.same_kind("ray_recurrence", gate, value=value)
+    if gate.dim() != 2 or value.shape != gate.shape or gate.shape[1] == 0:
+        raise _lib.EnvidrError(f"ray_recurrence: gate {tuple(gate.shape)} and value {tuple(value.shape)} are [T, C] both, C >= 1")
+    if rays.dim() != 2 or rays.shape[1] != 3 or rays.dtype != torch.int32 or rays.device != gate.device:
+        raise _lib.EnvidrError(f"ray_recurrence: rays is int32 [N, 3] on {gate.device}, not {rays.dtype} {tuple(rays.shape)} on {rays.device}")
+    if state is not None and (state.dtype != torch.float32 or state.shape != (rays.shape[0], gate.shape[1]) or state.device != gate.device):
+        raise _lib.EnvidrError(f"ray_recurrence: state is float32 [{rays.shape[0]}, {gate.shape[1]}] on {gate.device}, not {state.dtype} {tuple(state.shape)} on {state.device}")
+    gate, value, rays = gate.contiguous(), value.contiguous(), rays.contiguous()
+    state = None if state is None else state.contiguous()
+    if torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or state is not None and state.requires_grad):
+        return _RayRecurrence.apply(gate, value, state, rays, code, int(blend))
+    h, last, _ = _forward(gate, value, rays, state, code, int(blend), False)
+    return h, last
+
+
+def rays_of_lengths(lengths: torch.Tensor) -> torch.Tensor:
+    """`rays` int32 [N, 3] of N sequences packed one behind the other, from their lengths [N]"""
+    count = lengths.reshape(-1).to(torch.int64)
+    first = torch.cumsum(count, 0) - count
+    return torch.stack([torch.arange(count.shape[0], device=count.device), first, count], 1).to(torch.int32)

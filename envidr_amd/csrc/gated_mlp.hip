@@ -1,0 +1,641 @@
+// The gated feed-forward block  y = h Wd^T,  h = act(g) * u,  g = x Wg^T,  u = x Wu^T,  and its gradients.
+//
+//   forward   k_glu_forward  g and u in one tile (a wave holds the gate and the up column of the same hidden unit), act and product in the
+//                            epilogue, h stored once as the next product's operand
+//             k_product      y = h Wd^T
+//   backward  k_glu_backward g, u again and dh = dy Wd in one tile; dg = dh u act'(g), du = dh act(g) and h in the epilogue, from 32-bit values
+//             k_product      dx = dg Wg + du Wu (one reduction over 2 F)
+//             k_weight_grads dWg = dg^T x, dWu = du^T x, dWd = dy^T h: one launch, the reduction over the rows split where the results are too few
+//                            to fill the chip; partial sums in fp32, added in a fixed order
+// Why g and u are formed again: kept in 32 bits they cost 16 bytes a hidden unit of traffic, more than the 4 D flops of forming them while
+// D is below about 800; kept in 16 bits they would cost the gradients half a bit.
+//
+// Operands that the core cannot read as they are (fp32: three bf16 terms; widths, pitches or addresses that are no multiples of 16 bytes) are
+// laid out first by k_pack_operands.  Rows go in chunks of at most kChunkBytes of hidden-layer operands.
+//
+// Up to ENVIDR_GATED_FEW_ROWS rows the weights' bytes are all there is to move: k_few_rows streams them once through registers, sixteen
+// weight rows a workgroup, the reduction split over its waves.
+#include "gemm_core.hip.h"
+
+namespace envidr {
+namespace {
+
+// ---- layout of operands ----------------------------------------------------------------------------------------------------------------
+struct PackJob {
+    const void* src;
+    uint16_t* dst;
+    int64_t ld;
+    uint64_t plane;
+    uint32_t rows, cols, units;     // units = padded row / 8
+    uint32_t first_block;
+};
+struct PackJobs {
+    PackJob job[5];
+    uint32_t n;
+};
+
+template <class E, class T, int NP> __global__ void __launch_bounds__(kBlock) k_pack_operands(PackJobs a) {
+    uint32_t j = 0;
+    while (j + 1 < a.n && blockIdx.x >= a.job[j + 1].first_block) ++j;
+    const PackJob p = a.job[j];
+    const uint64_t at = (uint64_t)(blockIdx.x - p.first_block) * kBlock + threadIdx.x;
+    const uint64_t row = at / p.units;
+    if (row >= p.rows) return;
+    const uint32_t c0 = (uint32_t)(at % p.units) * 8u;
+    const E* s = static_cast<const E*>(p.src) + row * p.ld + c0;
+    float v[8];
+    if (c0 + 8u <= p.cols) {
+        const Pack<E, 8> x = load_pack<E, 8>(s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(x.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c0 + i < p.cols ? to_f32(s[i]) : 0.0f;
+    }
+    uint16_t* d = p.dst + (row * p.units + at % p.units) * 8u;
+    store_planes<T, NP>(d, p.plane, {v[0], v[1], v[2], v[3]});
+    store_planes<T, NP>(d + 4, p.plane, {v[4], v[5], v[6], v[7]});
+}
+
+// ---- tiles -----------------------------------------------------------------------------------------------------------------------------
+// Workgroups go to the eight XCDs in turn: each XCD gets a run of adjacent tiles, column tiles first, so that the rows of a run and the
+// weights stay in its own L2.
+__device__ __forceinline__ uint32_t tile_of(uint32_t block, uint32_t blocks) {
+    const uint32_t each = (blocks + 7u) / 8u;
+    return (block & 7u) * each + (block >> 3);
+}
+uint32_t padded_grid(uint64_t tiles) { return (uint32_t)((tiles + 7) / 8 * 8); }
+
+template <int NP> constexpr int k_step() { return NP == 1 ? 64 : 32; }
+
+struct GluArgs {
+    Operand x, wg, wu, dy, wd;
+    uint32_t M, F, D, O;            // D, O: the reductions, padded to 8
+    uint32_t Fp;
+    uint16_t *h, *dg, *du;          // [M][Fp] planes
+    uint64_t plane;
+    uint32_t col_tiles, tiles;
+};
+
+template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ void __launch_bounds__(WM* WN * 64) k_glu_forward(GluArgs a) {
+    using P = Product<T, NP, k_step<NP>(), TM, 2 * TF, WM, WN, true, true, true>;
+    __shared__ __attribute__((aligned(1024))) char lds0[P::kStage], lds1[P::kStage];
+    const uint32_t t = tile_of(blockIdx.x, a.tiles);
+    if (t >= a.tiles) return;
+    const uint32_t row0 = t / a.col_tiles * TM, f0 = t % a.col_tiles * TF;
+    f32x4 acc[P::MI][P::NI] = {};
+    P::run(a.x, a.wg, a.wu, row0, f0, 0, a.D, lds0, lds1, acc, 0);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+#pragma unroll
+    for (int mi = 0; mi < P::MI; ++mi) {
+        const uint32_t m = row0 + (wm * P::MI + mi) * 16u + (lane & 15u);
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int ni = 0; ni < P::NI; ni += 2) {
+            const uint32_t f = f0 + (wn * P::NI + ni) * 8u + 4u * (lane >> 4);
+            if (f >= a.Fp) continue;
+            float h[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float act, slope;
+                activation<ACT>(acc[mi][ni][r], act, slope);
+                h[r] = act * acc[mi][ni + 1][r];
+            }
+            store_planes<T, NP>(a.h + (uint64_t)m * a.Fp + f, a.plane, h);
+        }
+    }
+}
+
+template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ void __launch_bounds__(WM* WN * 64) k_glu_backward(GluArgs a) {
+    using P = Product<T, NP, k_step<NP>(), TM, 2 * TF, WM, WN, true, true, true>;
+    using Q = Product<T, NP, k_step<NP>(), TM, TF, WM, WN, true, false, false>;
+    __shared__ __attribute__((aligned(1024))) char lds0[P::kStage], lds1[P::kStage];
+    const uint32_t t = tile_of(blockIdx.x, a.tiles);
+    if (t >= a.tiles) return;
+    const uint32_t row0 = t / a.col_tiles * TM, f0 = t % a.col_tiles * TF;
+    f32x4 acc[P::MI][P::NI] = {}, dh[Q::MI][Q::NI] = {};
+    P::run(a.x, a.wg, a.wu, row0, f0, 0, a.D, lds0, lds1, acc, 0);
+    Q::run(a.dy, a.wd, a.wd, row0, f0, 0, a.O, lds0, lds1, dh, 0);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+#pragma unroll
+    for (int mi = 0; mi < P::MI; ++mi) {
+        const uint32_t m = row0 + (wm * P::MI + mi) * 16u + (lane & 15u);
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int ni = 0; ni < Q::NI; ++ni) {
+            const uint32_t f = f0 + (wn * Q::NI + ni) * 16u + 4u * (lane >> 4);
+            if (f >= a.Fp) continue;
+            float h[4], dg[4], du[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float act, slope;
+                const float u = acc[mi][2 * ni + 1][r], d = dh[mi][ni][r];
+                activation<ACT>(acc[mi][2 * ni][r], act, slope);
+                h[r] = act * u;
+                dg[r] = d * u * slope;
+                du[r] = d * act;
+            }
+            const uint64_t at = (uint64_t)m * a.Fp + f;
+            store_planes<T, NP>(a.h + at, a.plane, h);
+            store_planes<T, NP>(a.dg + at, a.plane, dg);
+            store_planes<T, NP>(a.du + at, a.plane, du);
+        }
+    }
+}
+
+struct ProductArgs {
+    Operand a[2], b[2];             // phases: the reduction runs over a[0] b[0], then a[1] b[1]
+    uint32_t K;
+    int phases;
+    void* out;
+    int64_t ld;
+    uint32_t M, N, col_tiles, tiles;
+};
+
+// rows x columns results of type E: BKC: b K-contiguous (y = h Wd^T), else K-strided (dx = dg Wg + du Wu)
+template <class E, class T, int NP, int TM, int TN, int WM, int WN, bool BKC> __global__ void __launch_bounds__(WM* WN * 64) k_product(ProductArgs a) {
+    using P = Product<T, NP, k_step<NP>(), TM, TN, WM, WN, true, BKC, false>;
+    __shared__ __attribute__((aligned(1024))) char lds0[P::kStage], lds1[P::kStage];
+    const uint32_t t = tile_of(blockIdx.x, a.tiles);
+    if (t >= a.tiles) return;
+    const uint32_t row0 = t / a.col_tiles * TM, col0 = t % a.col_tiles * TN;
+    f32x4 acc[P::MI][P::NI] = {};
+    for (int p = 0; p < a.phases; ++p) P::run(p ? a.a[1] : a.a[0], p ? a.b[1] : a.b[0], a.b[0], row0, col0, 0, a.K, lds0, lds1, acc, 0);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+    E* out = static_cast<E*>(a.out);
+#pragma unroll
+    for (int mi = 0; mi < P::MI; ++mi) {
+        const uint32_t m = row0 + (wm * P::MI + mi) * 16u + (lane & 15u);
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int ni = 0; ni < P::NI; ++ni) {
+            const uint32_t n = col0 + (wn * P::NI + ni) * 16u + 4u * (lane >> 4);
+            const float v[4] = {acc[mi][ni][0], acc[mi][ni][1], acc[mi][ni][2], acc[mi][ni][3]};
+            store_row4(out + (int64_t)m * a.ld + n, (int64_t)a.N - n, v);
+        }
+    }
+}
+
+struct GradJob {
+    Operand a, b;                   // both K-strided: result rows = a's columns
+    void* out;                      // [rows][cols], dense
+    float* part;                    // [splits][rows][cols] fp32, or NULL: the results go straight to `out`
+    uint32_t rows, cols, col_tiles, first_tile;
+};
+struct GradArgs {
+    GradJob job[3];
+    uint32_t jobs, K, per_split, splits, tiles;     // tiles: of one split
+    int add;                        // to what `part` holds (a later chunk of rows)
+};
+
+template <class E, class T, int NP, int TM, int TN, int WM, int WN> __global__ void __launch_bounds__(WM* WN * 64) k_weight_grads(GradArgs a) {
+    using P = Product<T, NP, k_step<NP>(), TM, TN, WM, WN, false, false, false>;
+    __shared__ __attribute__((aligned(1024))) char lds0[P::kStage], lds1[P::kStage];
+    const uint32_t all = a.tiles * a.splits, tt = tile_of(blockIdx.x, all);
+    if (tt >= all) return;
+    const uint32_t split = tt / a.tiles, t = tt % a.tiles;
+    uint32_t j = 0;
+    while (j + 1 < a.jobs && t >= a.job[j + 1].first_tile) ++j;
+    const GradJob& g = a.job[j];
+    const uint32_t i = t - g.first_tile, row0 = i / g.col_tiles * TM, col0 = i % g.col_tiles * TN;
+    const uint32_t from = min(split * a.per_split, a.K), to = min(from + a.per_split, a.K);
+    f32x4 acc[P::MI][P::NI] = {};
+    P::run(g.a, g.b, g.b, row0, col0, from, to, lds0, lds1, acc, 0);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+#pragma unroll
+    for (int mi = 0; mi < P::MI; ++mi) {
+        const uint32_t m = row0 + (wm * P::MI + mi) * 16u + (lane & 15u);
+        if (m >= g.rows) continue;
+#pragma unroll
+        for (int ni = 0; ni < P::NI; ++ni) {
+            const uint32_t n = col0 + (wn * P::NI + ni) * 16u + 4u * (lane >> 4);
+            float v[4] = {acc[mi][ni][0], acc[mi][ni][1], acc[mi][ni][2], acc[mi][ni][3]};
+            if (g.part) {
+                float* p = g.part + ((uint64_t)split * g.rows + m) * g.cols + n;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (a.add && n + r < g.cols) v[r] += p[r];
+                store_row4(p, (int64_t)g.cols - n, v);
+            } else {
+                store_row4(static_cast<E*>(g.out) + (uint64_t)m * g.cols + n, (int64_t)g.cols - n, v);
+            }
+        }
+    }
+}
+
+struct SumJob {
+    const float* part;
+    void* out;
+    uint64_t n;
+    uint32_t first_block;
+};
+struct SumArgs {
+    SumJob job[3];
+    uint32_t jobs, splits;
+};
+template <class E> __global__ void __launch_bounds__(kBlock) k_sum_splits(SumArgs a) {
+    uint32_t j = 0;
+    while (j + 1 < a.jobs && blockIdx.x >= a.job[j + 1].first_block) ++j;
+    const SumJob& s = a.job[j];
+    const uint64_t i = (uint64_t)(blockIdx.x - s.first_block) * kBlock + threadIdx.x;
+    if (i >= s.n) return;
+    float v = 0;
+    for (uint32_t k = 0; k < a.splits; ++k) v += s.part[k * s.n + i];
+    static_cast<E*>(s.out)[i] = from_f32<E>(v);
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------------------------------
+struct FewArgs {
+    const void *a, *w, *w2;
+    void* out;
+    int64_t lda, ldw, ldw2, ldo;
+    uint32_t M, K, N;
+};
+constexpr int kFewWaves = 8;
+
+// sixteen weight rows (of one or of both matrices) x all rows of a; every wave takes every kFewWaves-th step of the reduction
+template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWaves * 64) k_few_rows(FewArgs f) {
+    constexpr int W = 16 / sizeof(E);                    // elements of a lane's 16 bytes
+    constexpr uint32_t kStep = 4 * W;                    // k of a wave's step: four lane groups
+    constexpr int kMats = GLU ? 2 : 1;
+    __shared__ f32x4 part[kMats][kFewWaves][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15u, n0 = blockIdx.x * 16u;
+    const E* a = static_cast<const E*>(f.a) + (int64_t)min(i, f.M - 1u) * f.lda;
+    const uint32_t wr = min(n0 + i, f.N - 1u);
+    const E* w[kMats];
+    w[0] = static_cast<const E*>(f.w) + (int64_t)wr * f.ldw;
+    if constexpr (GLU) w[1] = static_cast<const E*>(f.w2) + (int64_t)wr * f.ldw2;
+    f32x4 acc[kMats] = {};
+    auto fetch = [&](const E* p, uint32_t k) {
+        if (k + W <= f.K) return load_pack<E, W>(p + k);
+        Pack<E, W> v;
+#pragma unroll
+        for (int q = 0; q < W; ++q) v.v[q] = k + q < f.K ? p[k + q] : from_f32<E>(0.0f);
+        return v;
+    };
+#pragma unroll 4
+    for (uint32_t k0 = wave * kStep; k0 < f.K; k0 += kFewWaves * kStep) {
+        const uint32_t k = k0 + g * W;
+        const Pack<E, W> x = fetch(a, k);
+#pragma unroll
+        for (int m = 0; m < kMats; ++m) {
+            const Pack<E, W> y = fetch(w[m], k);
+            if constexpr (sizeof(E) == 4) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(y.v[q], x.v[q], acc[m], 0, 0, 0);
+            } else {
+                acc[m] = mfma16<E>(__builtin_bit_cast(s16x8, y), __builtin_bit_cast(s16x8, x), acc[m]);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) part[m][wave][lane] = acc[m];
+    __syncthreads();
+    if (wave != 0 || i >= f.M) return;
+    f32x4 sum[kMats] = {};
+#pragma unroll
+    for (int m = 0; m < kMats; ++m)
+#pragma unroll
+        for (int q = 0; q < kFewWaves; ++q) sum[m] += part[m][q][lane];
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if constexpr (GLU) {
+            float act, slope;
+            activation<ACT>(sum[0][r], act, slope);
+            v[r] = act * sum[1][r];
+        } else {
+            v[r] = sum[0][r];
+        }
+    }
+    const uint32_t n = n0 + 4u * g;
+    store_row4(static_cast<E*>(f.out) + (int64_t)i * f.ldo + n, (int64_t)f.N - n, v);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+constexpr uint64_t kChunkBytes = 2ull << 30;    // of hidden-layer operands at a time
+constexpr uint32_t kMaxChunk = 1u << 22;        // rows (tile numbers stay within 32 bits at any width)
+constexpr uint32_t kMaxWidth = 1u << 20;
+
+uint32_t pad8(uint32_t v) { return (v + 7u) / 8u * 8u; }
+
+// where everything lies in the workspace, in bytes
+struct Plan {
+    uint32_t np, Dp, Fp, Op, chunk;
+    uint32_t splits, per_split;
+    uint64_t x, dy, wg, wu, wd, h, dg, du, part, bytes;
+};
+
+constexpr uint32_t kTile = 128;
+
+Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool backward) {
+    Plan p{};
+    p.np = dtype == ENVIDR_F32 ? 3u : 1u;
+    p.Dp = pad8(D);
+    p.Fp = pad8(F);
+    p.Op = pad8(O);
+    const uint64_t row = 2ull * p.np * p.Fp * (backward ? 3u : 1u);
+    const uint64_t most = kChunkBytes / row / 256u * 256u;
+    p.chunk = (uint32_t)(most < 256u ? 256u : (most < kMaxChunk ? most : kMaxChunk));
+    if (p.chunk > M) p.chunk = M;
+    if (!backward && M <= ENVIDR_GATED_FEW_ROWS) {
+        p.h = 0;
+        p.bytes = round_up64((uint64_t)M * p.Fp * dtype_size(dtype), 256);
+        return p;
+    }
+    uint64_t at = 0;
+    auto take = [&](uint64_t bytes) { const uint64_t here = at; at += round_up64(bytes, 256); return here; };
+    p.wg = take(2ull * p.np * F * p.Dp);
+    p.wu = take(2ull * p.np * F * p.Dp);
+    p.wd = take(2ull * p.np * O * p.Fp);
+    p.x = take(2ull * p.np * p.chunk * p.Dp);
+    p.h = take(2ull * p.np * p.chunk * p.Fp);
+    if (backward) {
+        p.dy = take(2ull * p.np * p.chunk * p.Op);
+        p.dg = take(2ull * p.np * p.chunk * p.Fp);
+        p.du = take(2ull * p.np * p.chunk * p.Fp);
+        // the rows' reduction is split until about two workgroups a CU are at work, in runs of 512 rows at least
+        const uint64_t tiles = 2ull * ceil_div(F, kTile) * ceil_div(D, kTile) + (uint64_t)ceil_div(O, kTile) * ceil_div(F, kTile);
+        uint64_t want = (512 + tiles - 1) / tiles;
+        const uint32_t can = ceil_div(p.chunk, 512u);
+        want = want < can ? want : can;
+        p.per_split = (uint32_t)round_up64(ceil_div(p.chunk, (uint32_t)want), 64);
+        p.splits = ceil_div(p.chunk, p.per_split);
+        if (p.splits > 1 || p.chunk < M) p.part = take(4ull * p.splits * (2ull * F * D + (uint64_t)O * F));
+    }
+    p.bytes = at;
+    return p;
+}
+
+struct Weights {
+    const void *wg, *wu, *wd;
+    int64_t lg, lu, ldn;
+};
+
+// can the core read it as it is: 16-byte rows of whole units
+bool readable(const void* p, int64_t ld, uint32_t cols, int dtype) {
+    return dtype != ENVIDR_F32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && cols % 8 == 0;
+}
+
+struct Packer {
+    PackJobs jobs{};
+    uint32_t blocks = 0;
+    int dtype;
+    uint32_t np;
+    // the operand for [rows, cols] at src: the tensor itself, or its place in the workspace and a job
+    Operand add(const void* src, int64_t ld, uint32_t rows, uint32_t cols, void* place, bool k_strided) {
+        const uint32_t units = pad8(cols) / 8u;
+        Operand o;
+        o.ext = k_strided ? units * 8u : rows;
+        if (readable(src, ld, cols, dtype)) {
+            o.p = static_cast<const uint16_t*>(src);
+            o.plane = 0;
+            o.ld = (uint32_t)ld;
+            return o;
+        }
+        o.p = static_cast<uint16_t*>(place);
+        o.ld = units * 8u;
+        o.plane = (uint64_t)rows * o.ld;
+        PackJob& j = jobs.job[jobs.n++];
+        j.src = src;
+        j.dst = static_cast<uint16_t*>(place);
+        j.ld = ld;
+        j.plane = o.plane;
+        j.rows = rows;
+        j.cols = cols;
+        j.units = units;
+        j.first_block = blocks;
+        blocks += (uint32_t)(((uint64_t)rows * units + kBlock - 1) / kBlock);
+        return o;
+    }
+    template <class E, class T, int NP> int launch(hipStream_t s) {
+        if (jobs.n == 0) return ENVIDR_OK;
+        hipLaunchKernelGGL((k_pack_operands<E, T, NP>), dim3(blocks), dim3(kBlock), 0, s, jobs);
+        return check_launch("k_pack_operands");
+    }
+};
+
+Operand hidden(const uint16_t* p, uint32_t Fp, uint32_t rows, uint64_t plane, bool k_strided) {
+    return {p, plane, Fp, k_strided ? Fp : rows};
+}
+
+#define ENVIDR_FOR_ACT(act, ACT, ...)                                                                  \
+    do {                                                                                               \
+        if ((act) == ENVIDR_ACT_SILU) { constexpr int ACT = ENVIDR_ACT_SILU; __VA_ARGS__; }            \
+        else if ((act) == ENVIDR_ACT_GELU) { constexpr int ACT = ENVIDR_ACT_GELU; __VA_ARGS__; }       \
+        else if ((act) == ENVIDR_ACT_RELU) { constexpr int ACT = ENVIDR_ACT_RELU; __VA_ARGS__; }       \
+        else { constexpr int ACT = ENVIDR_ACT_SIGMOID; __VA_ARGS__; }                                  \
+    } while (0)
+
+template <class E> struct Terms { using T = E; static constexpr int NP = 1; };
+template <> struct Terms<float> { using T = __bf16; static constexpr int NP = 3; };
+
+template <class E, bool BKC> int launch_product(ProductArgs a, hipStream_t s) {
+    using T = typename Terms<E>::T;
+    constexpr int NP = Terms<E>::NP;
+    a.col_tiles = ceil_div(a.N, 128u);
+    a.tiles = ceil_div(a.M, 128u) * a.col_tiles;
+    hipLaunchKernelGGL((k_product<E, T, NP, 128, 128, 2, 2, BKC>), dim3(padded_grid(a.tiles)), dim3(256), 0, s, a);
+    return check_launch("k_product");
+}
+
+template <class E> int forward(const void* x, int64_t ldx, const Weights& w, uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, int act,
+                               void* y, int64_t ldy, char* ws, hipStream_t s) {
+    using T = typename Terms<E>::T;
+    constexpr int NP = Terms<E>::NP;
+    const Plan p = make_plan(M, D, F, O, dtype, false);
+    if (M <= ENVIDR_GATED_FEW_ROWS) {
+        FewArgs f{x, w.wg, w.wu, ws, ldx, w.lg, w.lu, (int64_t)p.Fp, M, D, F};
+        ENVIDR_FOR_ACT(act, ACT, hipLaunchKernelGGL((k_few_rows<E, ACT, true>), dim3(ceil_div(F, 16u)), dim3(kFewWaves * 64), 0, s, f));
+        if (int rc = check_launch("k_few_rows")) return rc;
+        FewArgs d{ws, w.wd, nullptr, y, (int64_t)p.Fp, w.ldn, 0, ldy, M, F, O};
+        hipLaunchKernelGGL((k_few_rows<E, ENVIDR_ACT_SILU, false>), dim3(ceil_div(O, 16u)), dim3(kFewWaves * 64), 0, s, d);
+        return check_launch("k_few_rows");
+    }
+    Operand owg{}, owu{}, owd{};
+    for (uint32_t m0 = 0; m0 < M; m0 += p.chunk) {
+        const uint32_t rows = M - m0 < p.chunk ? M - m0 : p.chunk;
+        Packer pk;
+        pk.dtype = dtype;
+        pk.np = NP;
+        if (m0 == 0) {
+            owg = pk.add(w.wg, w.lg, F, D, ws + p.wg, false);
+            owu = pk.add(w.wu, w.lu, F, D, ws + p.wu, false);
+            owd = pk.add(w.wd, w.ldn, O, F, ws + p.wd, false);
+        }
+        const Operand ox = pk.add(static_cast<const E*>(x) + (int64_t)m0 * ldx, ldx, rows, D, ws + p.x, false);
+        if (int rc = pk.template launch<E, T, NP>(s)) return rc;
+        GluArgs a{};
+        a.x = ox; a.wg = owg; a.wu = owu;
+        a.M = rows; a.F = F; a.D = p.Dp; a.Fp = p.Fp;
+        a.h = reinterpret_cast<uint16_t*>(ws + p.h);
+        a.plane = (uint64_t)p.chunk * p.Fp;
+        a.col_tiles = ceil_div(F, 64u);
+        a.tiles = ceil_div(rows, 128u) * a.col_tiles;
+        ENVIDR_FOR_ACT(act, ACT, hipLaunchKernelGGL((k_glu_forward<T, NP, 128, 64, 2, 2, ACT>), dim3(padded_grid(a.tiles)), dim3(256), 0, s, a));
+        if (int rc = check_launch("k_glu_forward")) return rc;
+        ProductArgs q{};
+        q.a[0] = hidden(a.h, p.Fp, rows, a.plane, false);
+        q.b[0] = owd;
+        q.K = p.Fp; q.phases = 1;
+        q.out = static_cast<E*>(y) + (int64_t)m0 * ldy; q.ld = ldy; q.M = rows; q.N = O;
+        if (int rc = launch_product<E, true>(q, s)) return rc;
+    }
+    return ENVIDR_OK;
+}
+
+template <class E> int backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const Weights& w, uint32_t M, uint32_t D, uint32_t F, uint32_t O,
+                                int dtype, int act, void* dx, int64_t lddx, void* dwg, void* dwu, void* dwd, char* ws, hipStream_t s) {
+    using T = typename Terms<E>::T;
+    constexpr int NP = Terms<E>::NP;
+    const Plan p = make_plan(M, D, F, O, dtype, true);
+    Operand owg{}, owu{}, owd{};
+    float* part = p.part ? reinterpret_cast<float*>(ws + p.part) : nullptr;
+    auto strided = [](Operand o, uint32_t ext) { o.ext = ext; return o; };
+    for (uint32_t m0 = 0; m0 < M; m0 += p.chunk) {
+        const uint32_t rows = M - m0 < p.chunk ? M - m0 : p.chunk;
+        Packer pk;
+        pk.dtype = dtype;
+        pk.np = NP;
+        if (m0 == 0) {
+            owg = pk.add(w.wg, w.lg, F, D, ws + p.wg, false);
+            owu = pk.add(w.wu, w.lu, F, D, ws + p.wu, false);
+            owd = pk.add(w.wd, w.ldn, O, F, ws + p.wd, true);
+        }
+        const Operand ox = pk.add(static_cast<const E*>(x) + (int64_t)m0 * ldx, ldx, rows, D, ws + p.x, false);
+        const Operand ody = pk.add(static_cast<const E*>(dy) + (int64_t)m0 * lddy, lddy, rows, O, ws + p.dy, false);
+        if (int rc = pk.template launch<E, T, NP>(s)) return rc;
+        GluArgs a{};
+        a.x = ox; a.wg = owg; a.wu = owu; a.dy = ody; a.wd = owd;
+        a.M = rows; a.F = F; a.D = p.Dp; a.Fp = p.Fp;
+        a.O = O;                        // (the K-strided weights have O rows and no padding behind them)
+        a.h = reinterpret_cast<uint16_t*>(ws + p.h);
+        a.dg = reinterpret_cast<uint16_t*>(ws + p.dg);
+        a.du = reinterpret_cast<uint16_t*>(ws + p.du);
+        a.plane = (uint64_t)p.chunk * p.Fp;
+        a.col_tiles = ceil_div(F, 64u);
+        a.tiles = ceil_div(rows, 128u) * a.col_tiles;
+        ENVIDR_FOR_ACT(act, ACT, hipLaunchKernelGGL((k_glu_backward<T, NP, 128, 64, 2, 2, ACT>), dim3(padded_grid(a.tiles)), dim3(256), 0, s, a));
+        if (int rc = check_launch("k_glu_backward")) return rc;
+        if (dx) {
+            ProductArgs q{};
+            q.a[0] = hidden(a.dg, p.Fp, rows, a.plane, false);
+            q.a[1] = hidden(a.du, p.Fp, rows, a.plane, false);
+            q.b[0] = strided(owg, p.Dp);
+            q.b[1] = strided(owu, p.Dp);
+            q.K = F; q.phases = 2;
+            q.out = static_cast<E*>(dx) + (int64_t)m0 * lddx; q.ld = lddx; q.M = rows; q.N = D;
+            if (int rc = launch_product<E, false>(q, s)) return rc;
+        }
+        GradArgs g{};
+        auto job = [&](Operand l, Operand r, void* out, uint64_t part_at, uint32_t n_rows, uint32_t n_cols) {
+            if (!out) return;
+            GradJob& j = g.job[g.jobs++];
+            j.a = l; j.b = r; j.out = out; j.part = part ? part + part_at : nullptr;
+            j.rows = n_rows; j.cols = n_cols; j.col_tiles = ceil_div(n_cols, kTile);
+            j.first_tile = g.tiles;
+            g.tiles += ceil_div(n_rows, kTile) * j.col_tiles;
+        };
+        const uint64_t fd = (uint64_t)p.splits * F * D;
+        job(hidden(a.dg, p.Fp, rows, a.plane, true), strided(ox, p.Dp), dwg, 0, F, D);
+        job(hidden(a.du, p.Fp, rows, a.plane, true), strided(ox, p.Dp), dwu, fd, F, D);
+        job(strided(ody, p.Op), hidden(a.h, p.Fp, rows, a.plane, true), dwd, 2 * fd, O, F);
+        if (g.jobs) {
+            g.K = rows; g.per_split = p.per_split; g.splits = p.splits; g.add = m0 > 0;
+            hipLaunchKernelGGL((k_weight_grads<E, T, NP, 128, 128, 2, 2>), dim3(padded_grid((uint64_t)g.tiles * g.splits)), dim3(256), 0, s, g);
+            if (int rc = check_launch("k_weight_grads")) return rc;
+        }
+    }
+    if (part && (dwg || dwu || dwd)) {
+        SumArgs u{};
+        u.splits = p.splits;
+        uint32_t blocks = 0;
+        auto job = [&](void* out, uint64_t part_at, uint64_t n) {
+            if (!out) return;
+            u.job[u.jobs++] = {part + part_at, out, n, blocks};
+            blocks += (uint32_t)((n + kBlock - 1) / kBlock);
+        };
+        const uint64_t fd = (uint64_t)p.splits * F * D;
+        job(dwg, 0, (uint64_t)F * D);
+        job(dwu, fd, (uint64_t)F * D);
+        job(dwd, 2 * fd, (uint64_t)O * F);
+        hipLaunchKernelGGL((k_sum_splits<E>), dim3(blocks), dim3(kBlock), 0, s, u);
+        return check_launch("k_sum_splits");
+    }
+    return ENVIDR_OK;
+}
+
+__global__ void __launch_bounds__(kBlock) k_zero_bytes(uint16_t* p, uint64_t n) {
+    const uint64_t i = (uint64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (i < n) p[i] = 0;
+}
+
+int gated_checks(const char* what, uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, int activation) {
+    ENVIDR_REQUIRE(dtype_ok(dtype), "%s: unknown dtype %d", what, dtype);
+    ENVIDR_REQUIRE(activation >= ENVIDR_ACT_SILU && activation <= ENVIDR_ACT_SIGMOID, "%s: unknown activation %d", what, activation);
+    ENVIDR_REQUIRE(D >= 1 && F >= 1 && O >= 1 && D <= kMaxWidth && F <= kMaxWidth && O <= kMaxWidth, "%s: widths D=%u, F=%u, O=%u must be in 1 .. %u", what, D, F, O, kMaxWidth);
+    ENVIDR_REQUIRE(M <= 0x7FFFFF00u && (uint64_t)F * D <= 1ull << 32 && (uint64_t)O * F <= 1ull << 32, "%s: M=%u rows or a weight matrix of more than 2^32 elements", what, M);
+    return ENVIDR_OK;
+}
+
+int workspace_checks(const char* what, const void* workspace, uint64_t have, uint64_t need) {
+    ENVIDR_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && have >= need, "%s: workspace of %llu bytes, %llu needed (16-byte aligned)", what,
+                   (unsigned long long)have, (unsigned long long)need);
+    return ENVIDR_OK;
+}
+
+}  // namespace
+}  // namespace envidr
+
+using namespace envidr;
+
+extern "C" {
+
+uint64_t envidr_gated_mlp_workspace_bytes(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, int backward) {
+    if (M == 0 || gated_checks("gated_mlp", M, D, F, O, dtype, ENVIDR_ACT_SILU)) return 0;
+    return make_plan(M, D, F, O, dtype, backward != 0).bytes;
+}
+
+int envidr_gated_mlp_forward(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up,
+                             const void* w_down, int64_t ld_down, uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, int activation,
+                             void* y, int64_t ldy, void* workspace, uint64_t workspace_bytes, envidr_stream_t stream) {
+    if (int rc = gated_checks("gated_mlp_forward", M, D, F, O, dtype, activation)) return rc;
+    if (M == 0) return ENVIDR_OK;
+    ENVIDR_REQUIRE(x && w_gate && w_up && w_down && y, "gated_mlp_forward: null pointer");
+    const int64_t most = 1ll << 21;
+    ENVIDR_REQUIRE(ldx >= 0 && ld_gate >= 0 && ld_up >= 0 && ld_down >= 0 && ldx <= most && ld_gate <= most && ld_up <= most && ld_down <= most,
+                   "gated_mlp_forward: a row pitch is negative or above 2^21");
+    ENVIDR_REQUIRE(ldy >= O, "gated_mlp_forward: ldy=%lld < O=%u", (long long)ldy, O);
+    if (int rc = workspace_checks("gated_mlp_forward", workspace, workspace_bytes, envidr_gated_mlp_workspace_bytes(M, D, F, O, dtype, 0))) return rc;
+    const Weights w{w_gate, w_up, w_down, ld_gate, ld_up, ld_down};
+    ENVIDR_FOR_DTYPE(dtype, E, return forward<E>(x, ldx, w, M, D, F, O, dtype, activation, y, ldy, static_cast<char*>(workspace), as_stream(stream)));
+}
+
+int envidr_gated_mlp_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate,
+                              const void* w_up, int64_t ld_up, const void* w_down, int64_t ld_down, uint32_t M, uint32_t D, uint32_t F,
+                              uint32_t O, int dtype, int activation, void* dx, int64_t lddx, void* dw_gate, void* dw_up, void* dw_down,
+                              void* workspace, uint64_t workspace_bytes, envidr_stream_t stream) {
+    if (int rc = gated_checks("gated_mlp_backward", M, D, F, O, dtype, activation)) return rc;
+    hipStream_t s = as_stream(stream);
+    if (M == 0) {                                    // no rows: the weights' gradients are zero
+        void* out[3] = {dw_gate, dw_up, dw_down};
+        for (int i = 0; i < 3; ++i) {
+            if (!out[i]) continue;
+            const uint64_t n = (uint64_t)F * (i < 2 ? D : O) * (dtype_size(dtype) / 2u);
+            hipLaunchKernelGGL(k_zero_bytes, dim3((uint32_t)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, static_cast<uint16_t*>(out[i]), n);
+            if (int rc = check_launch("k_zero_bytes")) return rc;
+        }
+        return ENVIDR_OK;
+    }
+    ENVIDR_REQUIRE(dy && x && w_gate && w_up && w_down, "gated_mlp_backward: null pointer");
+    const int64_t most = 1ll << 21;
+    ENVIDR_REQUIRE(lddy >= 0 && ldx >= 0 && ld_gate >= 0 && ld_up >= 0 && ld_down >= 0 && lddy <= most && ldx <= most && ld_gate <= most && ld_up <= most && ld_down <= most,
+                   "gated_mlp_backward: a row pitch is negative or above 2^21");
+    ENVIDR_REQUIRE(!dx || lddx >= D, "gated_mlp_backward: lddx=%lld < D=%u", (long long)lddx, D);
+    if (int rc = workspace_checks("gated_mlp_backward", workspace, workspace_bytes, envidr_gated_mlp_workspace_bytes(M, D, F, O, dtype, 1))) return rc;
+    const Weights w{w_gate, w_up, w_down, ld_gate, ld_up, ld_down};
+    ENVIDR_FOR_DTYPE(dtype, E, return backward<E>(dy, lddy, x, ldx, w, M, D, F, O, dtype, activation, dx, lddx, dw_gate, dw_up, dw_down,
+                                                  static_cast<char*>(workspace), s));
+}
+
+}  // extern "C"
