@@ -58,87 +58,98 @@ template <class E, class T, int NP> __global__ void __launch_bounds__(kBlock) k_
 }
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------------------------
-// Workgroups go to the eight XCDs in turn: each XCD gets a run of adjacent tiles, column tiles first, so that the rows of a run and the
-// weights stay in its own L2.
-__device__ __forceinline__ uint32_t tile_of(uint32_t block, uint32_t blocks) {
-    const uint32_t each = (blocks + 7u) / 8u;
-    return (block & 7u) * each + (block >> 3);
-}
-uint32_t padded_grid(uint64_t tiles) { return (uint32_t)((tiles + 7) / 8 * 8); }
-
-template <int NP> constexpr int k_step() { return NP == 1 ? 64 : 32; }
+// The kernels below are persistent: as many workgroups as the chip holds at once walk the tiles, and the first two steps of a workgroup's next
+// product are loaded under the last two of the present one, before its results are stored.
 
 struct GluArgs {
     Operand x, wg, wu, dy, wd;
-    uint32_t M, F, D, O;            // D, O: the reductions, padded to 8
+    uint32_t M, F, D, O;            // D, O: the lengths of the reductions
     uint32_t Fp;
     uint16_t *h, *dg, *du;          // [M][Fp] planes
     uint64_t plane;
     uint32_t col_tiles, tiles;
 };
 
-template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ void __launch_bounds__(WM* WN * 64) k_glu_forward(GluArgs a) {
-    using P = Product<T, NP, k_step<NP>(), TM, 2 * TF, WM, WN, true, true, true>;
-    __shared__ __attribute__((aligned(1024))) char lds0[P::kStage], lds1[P::kStage];
-    const uint32_t t = tile_of(blockIdx.x, a.tiles);
-    if (t >= a.tiles) return;
-    const uint32_t row0 = t / a.col_tiles * TM, f0 = t % a.col_tiles * TF;
-    f32x4 acc[P::MI][P::NI] = {};
-    P::run(a.x, a.wg, a.wu, row0, f0, 0, a.D, lds0, lds1, acc, 0);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ void __launch_bounds__(WM* WN * 64, 2) k_glu_forward(GluArgs a) {
+    using P = Product<T, NP, TM, 2 * TF, WM, WN, true, true, true>;
+    using Out = PlaneStore<T, NP, P::NI * 8>;
+    constexpr int kStores = P::MI / Out::kBlocks * Out::kCount;
+    __shared__ __attribute__((aligned(1024))) char lds_all[2 * P::kStage + WM * WN * 2048];
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)lds_all, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), scratch = lds + 2 * P::kStage + wave * 2048u;
+    TileWalk walk(a.tiles);
+    if (!walk.valid()) return;
+    typename P::Source src;
+    const uint32_t n = P::steps(a.D);
+    auto aim = [&](uint32_t t) { src.init(a.x, a.wg, a.wu, t / a.col_tiles * TM, t % a.col_tiles * TF, 0, a.D); };
+    aim(walk.now);
+    src.issue(lds);
+    src.issue(lds + P::kStage);
+    uint32_t stage = 0;
+    for (bool fresh = true; walk.valid(); walk.now += walk.by, fresh = false) {
+        const uint32_t row0 = walk.now / a.col_tiles * TM + wave / WN * (P::MI * 16u), f0 = walk.now % a.col_tiles * TF + wave % WN * (P::NI * 8u);
+        const bool more = walk.more();
+        f32x4 acc[P::MI][P::NI] = {};
+        P::template run<kStores>(lds, P::kStage, stage, src, n, !fresh, acc, 0, [&] { if (more) aim(walk.now + walk.by); }, [&](uint32_t to) { if (more) src.issue(to); });
 #pragma unroll
-    for (int mi = 0; mi < P::MI; ++mi) {
-        const uint32_t m = row0 + (wm * P::MI + mi) * 16u + (lane & 15u);
-        if (m >= a.M) continue;
+        for (int mi = 0; mi < P::MI; mi += Out::kBlocks) {
+            float h[Out::kBlocks][P::NI / 2][4];
 #pragma unroll
-        for (int ni = 0; ni < P::NI; ni += 2) {
-            const uint32_t f = f0 + (wn * P::NI + ni) * 8u + 4u * (lane >> 4);
-            if (f >= a.Fp) continue;
-            float h[4];
+            for (int b = 0; b < Out::kBlocks; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float act, slope;
-                activation<ACT>(acc[mi][ni][r], act, slope);
-                h[r] = act * acc[mi][ni + 1][r];
-            }
-            store_planes<T, NP>(a.h + (uint64_t)m * a.Fp + f, a.plane, h);
+                for (int j = 0; j < P::NI / 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float act, slope;
+                        activation<ACT>(acc[mi + b][2 * j][r], act, slope);
+                        h[b][j][r] = act * acc[mi + b][2 * j + 1][r];
+                    }
+            Out::store(scratch, h, a.h, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
         }
     }
 }
 
-template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ void __launch_bounds__(WM* WN * 64) k_glu_backward(GluArgs a) {
-    using P = Product<T, NP, k_step<NP>(), TM, 2 * TF, WM, WN, true, true, true>;
-    using Q = Product<T, NP, k_step<NP>(), TM, TF, WM, WN, true, false, false>;
-    __shared__ __attribute__((aligned(1024))) char lds0[P::kStage], lds1[P::kStage];
-    const uint32_t t = tile_of(blockIdx.x, a.tiles);
-    if (t >= a.tiles) return;
-    const uint32_t row0 = t / a.col_tiles * TM, f0 = t % a.col_tiles * TF;
-    f32x4 acc[P::MI][P::NI] = {}, dh[Q::MI][Q::NI] = {};
-    P::run(a.x, a.wg, a.wu, row0, f0, 0, a.D, lds0, lds1, acc, 0);
-    Q::run(a.dy, a.wd, a.wd, row0, f0, 0, a.O, lds0, lds1, dh, 0);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ void __launch_bounds__(WM* WN * 64, 2) k_glu_backward(GluArgs a) {
+    using P = Product<T, NP, TM, 2 * TF, WM, WN, true, true, true>;
+    using Q = Product<T, NP, TM, TF, WM, WN, true, false, false>;
+    using Out = PlaneStore<T, NP, Q::NI * 16>;
+    constexpr int kStores = P::MI / Out::kBlocks * Out::kCount * 3;
+    __shared__ __attribute__((aligned(1024))) char lds_all[2 * P::kStage + WM * WN * 2048];
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)lds_all, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), scratch = lds + 2 * P::kStage + wave * 2048u;
+    TileWalk walk(a.tiles);
+    if (!walk.valid()) return;
+    typename P::Source src;
+    typename Q::Source src_h;
+    auto aim = [&](uint32_t t) { src.init(a.x, a.wg, a.wu, t / a.col_tiles * TM, t % a.col_tiles * TF, 0, a.D); };
+    aim(walk.now);
+    src.issue(lds);
+    src.issue(lds + P::kStage);
+    uint32_t stage = 0;
+    for (bool fresh = true; walk.valid(); walk.now += walk.by, fresh = false) {
+        const uint32_t tile_row = walk.now / a.col_tiles * TM, tile_col = walk.now % a.col_tiles * TF;
+        const uint32_t row0 = tile_row + wave / WN * (P::MI * 16u), f0 = tile_col + wave % WN * (Q::NI * 16u);
+        const bool more = walk.more();
+        f32x4 acc[P::MI][P::NI] = {}, dh[Q::MI][Q::NI] = {};
+        P::template run<kStores>(lds, P::kStage, stage, src, P::steps(a.D), !fresh, acc, 0, [&] { src_h.init(a.dy, a.wd, a.wd, tile_row, tile_col, 0, a.O); }, [&](uint32_t to) { src_h.issue(to); });
+        Q::template run<0>(lds, P::kStage, stage, src_h, Q::steps(a.O), false, dh, 0, [&] { if (more) aim(walk.now + walk.by); }, [&](uint32_t to) { if (more) src.issue(to); });
 #pragma unroll
-    for (int mi = 0; mi < P::MI; ++mi) {
-        const uint32_t m = row0 + (wm * P::MI + mi) * 16u + (lane & 15u);
-        if (m >= a.M) continue;
+        for (int mi = 0; mi < P::MI; mi += Out::kBlocks) {
+            float h[Out::kBlocks][Q::NI][4], dg[Out::kBlocks][Q::NI][4], du[Out::kBlocks][Q::NI][4];
 #pragma unroll
-        for (int ni = 0; ni < Q::NI; ++ni) {
-            const uint32_t f = f0 + (wn * Q::NI + ni) * 16u + 4u * (lane >> 4);
-            if (f >= a.Fp) continue;
-            float h[4], dg[4], du[4];
+            for (int b = 0; b < Out::kBlocks; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float act, slope;
-                const float u = acc[mi][2 * ni + 1][r], d = dh[mi][ni][r];
-                activation<ACT>(acc[mi][2 * ni][r], act, slope);
-                h[r] = act * u;
-                dg[r] = d * u * slope;
-                du[r] = d * act;
-            }
-            const uint64_t at = (uint64_t)m * a.Fp + f;
-            store_planes<T, NP>(a.h + at, a.plane, h);
-            store_planes<T, NP>(a.dg + at, a.plane, dg);
-            store_planes<T, NP>(a.du + at, a.plane, du);
+                for (int j = 0; j < Q::NI; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float act, slope;
+                        const float u = acc[mi + b][2 * j + 1][r], d = dh[mi + b][j][r];
+                        activation<ACT>(acc[mi + b][2 * j][r], act, slope);
+                        h[b][j][r] = act * u;
+                        dg[b][j][r] = d * u * slope;
+                        du[b][j][r] = d * act;
+                    }
+            Out::store(scratch, h, a.h, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
+            Out::store(scratch, dg, a.dg, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
+            Out::store(scratch, du, a.du, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
         }
     }
 }
@@ -146,33 +157,37 @@ template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ v
 struct ProductArgs {
     Operand a[2], b[2];             // phases: the reduction runs over a[0] b[0], then a[1] b[1]
     uint32_t K;
-    int phases;
+    uint32_t phases;
     void* out;
     int64_t ld;
     uint32_t M, N, col_tiles, tiles;
+    bool aligned;
 };
 
 // rows x columns results of type E: BKC: b K-contiguous (y = h Wd^T), else K-strided (dx = dg Wg + du Wu)
-template <class E, class T, int NP, int TM, int TN, int WM, int WN, bool BKC> __global__ void __launch_bounds__(WM* WN * 64) k_product(ProductArgs a) {
-    using P = Product<T, NP, k_step<NP>(), TM, TN, WM, WN, true, BKC, false>;
-    __shared__ __attribute__((aligned(1024))) char lds0[P::kStage], lds1[P::kStage];
-    const uint32_t t = tile_of(blockIdx.x, a.tiles);
-    if (t >= a.tiles) return;
-    const uint32_t row0 = t / a.col_tiles * TM, col0 = t % a.col_tiles * TN;
-    f32x4 acc[P::MI][P::NI] = {};
-    for (int p = 0; p < a.phases; ++p) P::run(p ? a.a[1] : a.a[0], p ? a.b[1] : a.b[0], a.b[0], row0, col0, 0, a.K, lds0, lds1, acc, 0);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-    E* out = static_cast<E*>(a.out);
-#pragma unroll
-    for (int mi = 0; mi < P::MI; ++mi) {
-        const uint32_t m = row0 + (wm * P::MI + mi) * 16u + (lane & 15u);
-        if (m >= a.M) continue;
-#pragma unroll
-        for (int ni = 0; ni < P::NI; ++ni) {
-            const uint32_t n = col0 + (wn * P::NI + ni) * 16u + 4u * (lane >> 4);
-            const float v[4] = {acc[mi][ni][0], acc[mi][ni][1], acc[mi][ni][2], acc[mi][ni][3]};
-            store_row4(out + (int64_t)m * a.ld + n, (int64_t)a.N - n, v);
+template <class E, class T, int NP, int TM, int TN, int WM, int WN, bool BKC> __global__ void __launch_bounds__(WM* WN * 64, 2) k_product(ProductArgs a) {
+    using P = Product<T, NP, TM, TN, WM, WN, true, BKC, false>;
+    using Out = ResultStore<E, P::MI, P::NI>;
+    __shared__ __attribute__((aligned(1024))) char lds_all[2 * P::kStage + (Out::kWide ? 0 : WM * WN * 2048)];
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)lds_all, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), scratch = lds + 2 * P::kStage + wave * 2048u;
+    TileWalk walk(a.tiles);
+    if (!walk.valid()) return;
+    typename P::Source src;
+    const uint32_t n = P::steps(a.K);
+    auto aim = [&](uint32_t t, uint32_t p) { src.init(p ? a.a[1] : a.a[0], p ? a.b[1] : a.b[0], a.b[0], t / a.col_tiles * TM, t % a.col_tiles * TN, 0, a.K); };
+    aim(walk.now, 0);
+    src.issue(lds);
+    src.issue(lds + P::kStage);
+    uint32_t stage = 0;
+    for (bool fresh = true; walk.valid(); walk.now += walk.by, fresh = false) {
+        const bool more = walk.more();
+        f32x4 acc[P::MI][P::NI] = {};
+        for (uint32_t p = 0; p < a.phases; ++p) {
+            const bool goes_on = more || p + 1 < a.phases;
+            P::template run<Out::kCount>(lds, P::kStage, stage, src, n, !fresh && a.aligned && p == 0, acc, 0,
+                                         [&] { if (p + 1 < a.phases) aim(walk.now, p + 1); else if (more) aim(walk.now + walk.by, 0); }, [&](uint32_t to) { if (goes_on) src.issue(to); });
         }
+        Out::store(scratch, acc, static_cast<E*>(a.out), a.ld, a.M, a.N, walk.now / a.col_tiles * TM + wave / WN * (P::MI * 16u), walk.now % a.col_tiles * TN + wave % WN * (P::NI * 16u), a.aligned);
     }
 }
 
@@ -181,45 +196,67 @@ struct GradJob {
     void* out;                      // [rows][cols], dense
     float* part;                    // [splits][rows][cols] fp32, or NULL: the results go straight to `out`
     uint32_t rows, cols, col_tiles, first_tile;
+    bool aligned;
 };
 struct GradArgs {
     GradJob job[3];
     uint32_t jobs, K, per_split, splits, tiles;     // tiles: of one split
-    int add;                        // to what `part` holds (a later chunk of rows)
+    bool add;                       // to what `part` holds (a later chunk of rows)
 };
 
-template <class E, class T, int NP, int TM, int TN, int WM, int WN> __global__ void __launch_bounds__(WM* WN * 64) k_weight_grads(GradArgs a) {
-    using P = Product<T, NP, k_step<NP>(), TM, TN, WM, WN, false, false, false>;
-    __shared__ __attribute__((aligned(1024))) char lds0[P::kStage], lds1[P::kStage];
-    const uint32_t all = a.tiles * a.splits, tt = tile_of(blockIdx.x, all);
-    if (tt >= all) return;
-    const uint32_t split = tt / a.tiles, t = tt % a.tiles;
-    uint32_t j = 0;
-    while (j + 1 < a.jobs && t >= a.job[j + 1].first_tile) ++j;
-    const GradJob& g = a.job[j];
-    const uint32_t i = t - g.first_tile, row0 = i / g.col_tiles * TM, col0 = i % g.col_tiles * TN;
-    const uint32_t from = min(split * a.per_split, a.K), to = min(from + a.per_split, a.K);
-    f32x4 acc[P::MI][P::NI] = {};
-    P::run(g.a, g.b, g.b, row0, col0, from, to, lds0, lds1, acc, 0);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-#pragma unroll
-    for (int mi = 0; mi < P::MI; ++mi) {
-        const uint32_t m = row0 + (wm * P::MI + mi) * 16u + (lane & 15u);
-        if (m >= g.rows) continue;
-#pragma unroll
-        for (int ni = 0; ni < P::NI; ++ni) {
-            const uint32_t n = col0 + (wn * P::NI + ni) * 16u + 4u * (lane >> 4);
-            float v[4] = {acc[mi][ni][0], acc[mi][ni][1], acc[mi][ni][2], acc[mi][ni][3]};
-            if (g.part) {
-                float* p = g.part + ((uint64_t)split * g.rows + m) * g.cols + n;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (a.add && n + r < g.cols) v[r] += p[r];
-                store_row4(p, (int64_t)g.cols - n, v);
-            } else {
-                store_row4(static_cast<E*>(g.out) + (uint64_t)m * g.cols + n, (int64_t)g.cols - n, v);
-            }
+template <class E, class T, int NP, int TM, int TN, int WM, int WN> __global__ void __launch_bounds__(WM* WN * 64, 2) k_weight_grads(GradArgs a) {
+    using P = Product<T, NP, TM, TN, WM, WN, false, false, false>;
+    using Part = ResultStore<float, P::MI, P::NI>;
+    using Out = ResultStore<E, P::MI, P::NI>;
+    __shared__ __attribute__((aligned(1024))) char lds_all[2 * P::kStage + (Out::kWide ? 0 : WM * WN * 2048)];
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)lds_all, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), scratch = lds + 2 * P::kStage + wave * 2048u;
+    TileWalk walk(a.tiles * a.splits);
+    if (!walk.valid()) return;
+    struct Spot { uint32_t split, j, row0, col0, from, to; };
+    auto spot = [&](uint32_t tt) {
+        Spot s;
+        s.split = tt / a.tiles;
+        const uint32_t t = tt % a.tiles;
+        s.j = 0;
+        while (s.j + 1 < a.jobs && t >= a.job[s.j + 1].first_tile) ++s.j;
+        const uint32_t i = t - a.job[s.j].first_tile;
+        s.row0 = i / a.job[s.j].col_tiles * TM;
+        s.col0 = i % a.job[s.j].col_tiles * TN;
+        s.from = min(s.split * a.per_split, a.K);
+        s.to = min(s.from + a.per_split, a.K);
+        return s;
+    };
+    typename P::Source src;
+    auto aim = [&](const Spot& s) { src.init(a.job[s.j].a, a.job[s.j].b, a.job[s.j].b, s.row0, s.col0, s.from, s.to); };
+    Spot now = spot(walk.now), next = now;
+    aim(now);
+    src.issue(lds);
+    src.issue(lds + P::kStage);
+    uint32_t stage = 0;
+    for (; walk.valid(); walk.now += walk.by, now = next) {
+        const bool more = walk.more();
+        f32x4 acc[P::MI][P::NI] = {};
+        P::template run<0>(lds, P::kStage, stage, src, P::steps(now.to - now.from), false, acc, 0, [&] { if (more) { next = spot(walk.now + walk.by); aim(next); } }, [&](uint32_t to) { if (more) src.issue(to); });
+        const GradJob& g = a.job[now.j];
+        const uint32_t row0 = now.row0 + wave / WN * (P::MI * 16u), col0 = now.col0 + wave % WN * (P::NI * 16u);
+        if (!g.part) {
+            Out::store(scratch, acc, static_cast<E*>(g.out), g.cols, g.rows, g.cols, row0, col0, g.aligned);
+            continue;
         }
+        float* part = g.part + (uint64_t)now.split * g.rows * g.cols;
+        if (a.add) {
+            const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+            for (int mi = 0; mi < P::MI; ++mi)
+#pragma unroll
+                for (int ni = 0; ni < P::NI; ++ni) {
+                    const uint32_t m = row0 + mi * 16u + (lane & 15u), n = col0 + ni * 16u + 4u * (lane >> 4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m < g.rows && n + r < g.cols) acc[mi][ni][r] += part[(uint64_t)m * g.cols + n + r];
+                }
+        }
+        Part::store(scratch, acc, part, g.cols, g.rows, g.cols, row0, col0, g.cols % 4u == 0);
     }
 }
 
@@ -273,7 +310,6 @@ template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWave
         for (int q = 0; q < W; ++q) v.v[q] = k + q < f.K ? p[k + q] : from_f32<E>(0.0f);
         return v;
     };
-#pragma unroll 4
     for (uint32_t k0 = wave * kStep; k0 < f.K; k0 += kFewWaves * kStep) {
         const uint32_t k = k0 + g * W;
         const Pack<E, W> x = fetch(a, k);
@@ -323,10 +359,26 @@ uint32_t pad8(uint32_t v) { return (v + 7u) / 8u * 8u; }
 struct Plan {
     uint32_t np, Dp, Fp, Op, chunk;
     uint32_t splits, per_split;
+    bool large_grads;
     uint64_t x, dy, wg, wu, wd, h, dg, du, part, bytes;
 };
 
-constexpr uint32_t kTile = 128;
+// Tiles.  Large: 256 x 256 by eight waves, one workgroup a CU -- LDS reads take 3/4 of the products' time where 128 x 128 by four waves takes
+// all of it (32 768 x 4096 x 1024, bf16: 1060 against 780 TFLOP/s).  The three terms of fp32 fill the LDS with 256 x 128, and six products a
+// pair of reads leave the reads' share below half.  Small where the large tiles are fewer than 3/4 of the CUs.
+constexpr uint32_t kCus = 256, kEnoughTiles = 192;
+struct TileSize {
+    uint32_t m, n;
+};
+uint64_t tiles_of(uint64_t rows, uint64_t cols, TileSize t) { return (rows + t.m - 1) / t.m * ((cols + t.n - 1) / t.n); }
+constexpr TileSize product_tile(uint32_t np, bool large) { return large ? (np == 1 ? TileSize{256, 256} : TileSize{256, 128}) : TileSize{128, 128}; }
+bool large_product(uint64_t rows, uint64_t cols, uint32_t np) { return tiles_of(rows, cols, product_tile(np, true)) >= kEnoughTiles; }
+uint64_t grad_tiles(uint32_t D, uint32_t F, uint32_t O, TileSize t) { return 2 * tiles_of(F, D, t) + tiles_of(O, F, t); }
+// workgroups: as many as are resident at once, in whole rounds of the XCDs
+uint32_t grid_of(uint64_t tiles, uint32_t per_cu) {
+    const uint64_t all = (tiles + 7) / 8 * 8, most = (uint64_t)kCus * per_cu;
+    return (uint32_t)(all < most ? all : most);
+}
 
 Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool backward) {
     Plan p{};
@@ -354,12 +406,26 @@ Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool b
         p.dy = take(2ull * p.np * p.chunk * p.Op);
         p.dg = take(2ull * p.np * p.chunk * p.Fp);
         p.du = take(2ull * p.np * p.chunk * p.Fp);
-        // the rows' reduction is split until about two workgroups a CU are at work, in runs of 512 rows at least
-        const uint64_t tiles = 2ull * ceil_div(F, kTile) * ceil_div(D, kTile) + (uint64_t)ceil_div(O, kTile) * ceil_div(F, kTile);
-        uint64_t want = (512 + tiles - 1) / tiles;
-        const uint32_t can = ceil_div(p.chunk, 512u);
-        want = want < can ? want : can;
-        p.per_split = (uint32_t)round_up64(ceil_div(p.chunk, (uint32_t)want), 64);
+        // The rows' reduction is split where the results alone do not fill the chip.  Of the numbers of parts (of 512 rows at least) the one
+        // whose rounds of tiles cost least, with what its partial sums cost to write and read again: in 1e-9 ms, a round of the products at
+        // about 1000 TFLOP/s and a result's 8 bytes at 4 TB/s.
+        const double results = 2.0 * F * D + (double)O * F, per_part = results * 2e-3;
+        const uint32_t can = ceil_div(p.chunk, 512u), most_parts = can < 64u ? can : 64u;
+        double best = 0;
+        for (int large = 0; large < 2; ++large) {
+            const TileSize tile = product_tile(p.np, large);
+            const double tiles = (double)grad_tiles(D, F, O, tile), slots = kCus * (large || p.np > 1 ? 1.0 : 2.0);
+            const double one_tile = 2.0 * p.chunk * tile.m * tile.n * (p.np == 3 ? 6 : 1) * slots / (large ? 1000.0 : 750.0);          // all rows of it, on its slot
+            for (uint32_t s = 1; s <= most_parts; ++s) {
+                const double cost = __builtin_ceil(tiles * s / slots) * one_tile / s + (s > 1 ? s * per_part : 0.0);
+                if (best == 0 || cost < best) {
+                    best = cost;
+                    p.large_grads = large;
+                    p.splits = s;
+                }
+            }
+        }
+        p.per_split = (uint32_t)round_up64(ceil_div(p.chunk, p.splits), 64);
         p.splits = ceil_div(p.chunk, p.per_split);
         if (p.splits > 1 || p.chunk < M) p.part = take(4ull * p.splits * (2ull * F * D + (uint64_t)O * F));
     }
@@ -430,13 +496,71 @@ Operand hidden(const uint16_t* p, uint32_t Fp, uint32_t rows, uint64_t plane, bo
 template <class E> struct Terms { using T = E; static constexpr int NP = 1; };
 template <> struct Terms<float> { using T = __bf16; static constexpr int NP = 3; };
 
-template <class E, bool BKC> int launch_product(ProductArgs a, hipStream_t s) {
+template <class E, int TM, int TN, int WM, int WN, bool BKC> int launch_product_as(ProductArgs a, hipStream_t s) {
     using T = typename Terms<E>::T;
     constexpr int NP = Terms<E>::NP;
-    a.col_tiles = ceil_div(a.N, 128u);
-    a.tiles = ceil_div(a.M, 128u) * a.col_tiles;
-    hipLaunchKernelGGL((k_product<E, T, NP, 128, 128, 2, 2, BKC>), dim3(padded_grid(a.tiles)), dim3(256), 0, s, a);
+    a.col_tiles = ceil_div(a.N, (uint32_t)TN);
+    a.tiles = ceil_div(a.M, (uint32_t)TM) * a.col_tiles;
+    hipLaunchKernelGGL((k_product<E, T, NP, TM, TN, WM, WN, BKC>), dim3(grid_of(a.tiles, WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
     return check_launch("k_product");
+}
+bool whole_units(const void* p, int64_t ld, uint32_t cols, uint32_t size) {
+    const uint32_t unit = 16u / size;
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % unit == 0 && cols % unit == 0;
+}
+template <class E, bool BKC> int launch_product(ProductArgs a, hipStream_t s) {
+    constexpr int NP = Terms<E>::NP;
+    a.aligned = whole_units(a.out, a.ld, a.N, sizeof(E));
+    if (!large_product(a.M, a.N, NP)) return launch_product_as<E, 128, 128, 2, 2, BKC>(a, s);
+    if constexpr (NP == 1) return launch_product_as<E, 256, 256, 2, 4, BKC>(a, s);
+    else return launch_product_as<E, 256, 128, 4, 2, BKC>(a, s);
+}
+
+template <class E, int ACT, int TM, int TF, int WM, int WN> int launch_glu_forward_as(GluArgs a, hipStream_t s) {
+    using T = typename Terms<E>::T;
+    constexpr int NP = Terms<E>::NP;
+    a.col_tiles = ceil_div(a.F, (uint32_t)TF);
+    a.tiles = ceil_div(a.M, (uint32_t)TM) * a.col_tiles;
+    hipLaunchKernelGGL((k_glu_forward<T, NP, TM, TF, WM, WN, ACT>), dim3(grid_of(a.tiles, WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
+    return check_launch("k_glu_forward");
+}
+template <class E, int ACT> int launch_glu_forward(const GluArgs& a, hipStream_t s) {
+    constexpr int NP = Terms<E>::NP;
+    if (!large_product(a.M, 2ull * a.F, NP)) return launch_glu_forward_as<E, ACT, 128, 64, 2, 2>(a, s);
+    if constexpr (NP == 1) return launch_glu_forward_as<E, ACT, 256, 128, 2, 4>(a, s);
+    else return launch_glu_forward_as<E, ACT, 256, 64, 4, 2>(a, s);
+}
+
+template <class E, int ACT, int TM, int TF, int WM, int WN> int launch_glu_backward_as(GluArgs a, hipStream_t s) {
+    using T = typename Terms<E>::T;
+    constexpr int NP = Terms<E>::NP;
+    a.col_tiles = ceil_div(a.F, (uint32_t)TF);
+    a.tiles = ceil_div(a.M, (uint32_t)TM) * a.col_tiles;
+    hipLaunchKernelGGL((k_glu_backward<T, NP, TM, TF, WM, WN, ACT>), dim3(grid_of(a.tiles, WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
+    return check_launch("k_glu_backward");
+}
+// (three accumulators a hidden unit: half the columns of the other products)
+template <class E, int ACT> int launch_glu_backward(const GluArgs& a, hipStream_t s) {
+    constexpr int NP = Terms<E>::NP;
+    if constexpr (NP == 1) {
+        if (tiles_of(a.M, a.F, {256, 64}) >= kEnoughTiles) return launch_glu_backward_as<E, ACT, 256, 64, 4, 2>(a, s);
+        return launch_glu_backward_as<E, ACT, 128, 64, 2, 2>(a, s);
+    } else {
+        return launch_glu_backward_as<E, ACT, 128, 64, 4, 2>(a, s);
+    }
+}
+
+template <class E, int TM, int TN, int WM, int WN> int launch_weight_grads_as(const GradArgs& a, hipStream_t s) {
+    using T = typename Terms<E>::T;
+    constexpr int NP = Terms<E>::NP;
+    hipLaunchKernelGGL((k_weight_grads<E, T, NP, TM, TN, WM, WN>), dim3(grid_of((uint64_t)a.tiles * a.splits, WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
+    return check_launch("k_weight_grads");
+}
+template <class E> int launch_weight_grads(const GradArgs& a, bool large, hipStream_t s) {
+    constexpr int NP = Terms<E>::NP;
+    if (!large) return launch_weight_grads_as<E, 128, 128, 2, 2>(a, s);
+    if constexpr (NP == 1) return launch_weight_grads_as<E, 256, 256, 2, 4>(a, s);
+    else return launch_weight_grads_as<E, 256, 128, 4, 2>(a, s);
 }
 
 template <class E> int forward(const void* x, int64_t ldx, const Weights& w, uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, int act,
@@ -470,10 +594,7 @@ template <class E> int forward(const void* x, int64_t ldx, const Weights& w, uin
         a.M = rows; a.F = F; a.D = p.Dp; a.Fp = p.Fp;
         a.h = reinterpret_cast<uint16_t*>(ws + p.h);
         a.plane = (uint64_t)p.chunk * p.Fp;
-        a.col_tiles = ceil_div(F, 64u);
-        a.tiles = ceil_div(rows, 128u) * a.col_tiles;
-        ENVIDR_FOR_ACT(act, ACT, hipLaunchKernelGGL((k_glu_forward<T, NP, 128, 64, 2, 2, ACT>), dim3(padded_grid(a.tiles)), dim3(256), 0, s, a));
-        if (int rc = check_launch("k_glu_forward")) return rc;
+        ENVIDR_FOR_ACT(act, ACT, if (int rc = (launch_glu_forward<E, ACT>(a, s))) return rc);
         ProductArgs q{};
         q.a[0] = hidden(a.h, p.Fp, rows, a.plane, false);
         q.b[0] = owd;
@@ -513,10 +634,7 @@ template <class E> int backward(const void* dy, int64_t lddy, const void* x, int
         a.dg = reinterpret_cast<uint16_t*>(ws + p.dg);
         a.du = reinterpret_cast<uint16_t*>(ws + p.du);
         a.plane = (uint64_t)p.chunk * p.Fp;
-        a.col_tiles = ceil_div(F, 64u);
-        a.tiles = ceil_div(rows, 128u) * a.col_tiles;
-        ENVIDR_FOR_ACT(act, ACT, hipLaunchKernelGGL((k_glu_backward<T, NP, 128, 64, 2, 2, ACT>), dim3(padded_grid(a.tiles)), dim3(256), 0, s, a));
-        if (int rc = check_launch("k_glu_backward")) return rc;
+        ENVIDR_FOR_ACT(act, ACT, if (int rc = (launch_glu_backward<E, ACT>(a, s))) return rc);
         if (dx) {
             ProductArgs q{};
             q.a[0] = hidden(a.dg, p.Fp, rows, a.plane, false);
@@ -532,9 +650,11 @@ template <class E> int backward(const void* dy, int64_t lddy, const void* x, int
             if (!out) return;
             GradJob& j = g.job[g.jobs++];
             j.a = l; j.b = r; j.out = out; j.part = part ? part + part_at : nullptr;
-            j.rows = n_rows; j.cols = n_cols; j.col_tiles = ceil_div(n_cols, kTile);
+            const TileSize tile = product_tile(NP, p.large_grads);
+            j.rows = n_rows; j.cols = n_cols; j.col_tiles = ceil_div(n_cols, tile.n);
             j.first_tile = g.tiles;
-            g.tiles += ceil_div(n_rows, kTile) * j.col_tiles;
+            j.aligned = whole_units(out, n_cols, n_cols, sizeof(E));
+            g.tiles += ceil_div(n_rows, tile.m) * j.col_tiles;
         };
         const uint64_t fd = (uint64_t)p.splits * F * D;
         job(hidden(a.dg, p.Fp, rows, a.plane, true), strided(ox, p.Dp), dwg, 0, F, D);
@@ -542,8 +662,7 @@ template <class E> int backward(const void* dy, int64_t lddy, const void* x, int
         job(strided(ody, p.Op), hidden(a.h, p.Fp, rows, a.plane, true), dwd, 2 * fd, O, F);
         if (g.jobs) {
             g.K = rows; g.per_split = p.per_split; g.splits = p.splits; g.add = m0 > 0;
-            hipLaunchKernelGGL((k_weight_grads<E, T, NP, 128, 128, 2, 2>), dim3(padded_grid((uint64_t)g.tiles * g.splits)), dim3(256), 0, s, g);
-            if (int rc = check_launch("k_weight_grads")) return rc;
+            if (int rc = launch_weight_grads<E>(g, p.large_grads, s)) return rc;
         }
     }
     if (part && (dwg || dwu || dwd)) {
@@ -605,7 +724,7 @@ int envidr_gated_mlp_forward(const void* x, int64_t ldx, const void* w_gate, int
     const int64_t most = 1ll << 21;
     ENVIDR_REQUIRE(ldx >= 0 && ld_gate >= 0 && ld_up >= 0 && ld_down >= 0 && ldx <= most && ld_gate <= most && ld_up <= most && ld_down <= most,
                    "gated_mlp_forward: a row pitch is negative or above 2^21");
-    ENVIDR_REQUIRE(ldy >= O, "gated_mlp_forward: ldy=%lld < O=%u", (long long)ldy, O);
+    ENVIDR_REQUIRE(ldy >= O && ldy <= most, "gated_mlp_forward: ldy=%lld < O=%u, or above 2^21", (long long)ldy, O);
     if (int rc = workspace_checks("gated_mlp_forward", workspace, workspace_bytes, envidr_gated_mlp_workspace_bytes(M, D, F, O, dtype, 0))) return rc;
     const Weights w{w_gate, w_up, w_down, ld_gate, ld_up, ld_down};
     ENVIDR_FOR_DTYPE(dtype, E, return forward<E>(x, ldx, w, M, D, F, O, dtype, activation, y, ldy, static_cast<char*>(workspace), as_stream(stream)));
@@ -631,7 +750,7 @@ int envidr_gated_mlp_backward(const void* dy, int64_t lddy, const void* x, int64
     const int64_t most = 1ll << 21;
     ENVIDR_REQUIRE(lddy >= 0 && ldx >= 0 && ld_gate >= 0 && ld_up >= 0 && ld_down >= 0 && lddy <= most && ldx <= most && ld_gate <= most && ld_up <= most && ld_down <= most,
                    "gated_mlp_backward: a row pitch is negative or above 2^21");
-    ENVIDR_REQUIRE(!dx || lddx >= D, "gated_mlp_backward: lddx=%lld < D=%u", (long long)lddx, D);
+    ENVIDR_REQUIRE(!dx || (lddx >= D && lddx <= most), "gated_mlp_backward: lddx=%lld < D=%u, or above 2^21", (long long)lddx, D);
     if (int rc = workspace_checks("gated_mlp_backward", workspace, workspace_bytes, envidr_gated_mlp_workspace_bytes(M, D, F, O, dtype, 1))) return rc;
     const Weights w{w_gate, w_up, w_down, ld_gate, ld_up, ld_down};
     ENVIDR_FOR_DTYPE(dtype, E, return backward<E>(dy, lddy, x, ldx, w, M, D, F, O, dtype, activation, dx, lddx, dw_gate, dw_up, dw_down,

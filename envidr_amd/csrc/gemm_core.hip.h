@@ -15,12 +15,18 @@
 #pragma once
 #include "blocks_common.hip.h"
 
+// (an LDS pointer is 32 bits on the device; the compiler's host pass warns about its own 64)
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"
+
 namespace envidr {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) s16x8 lds_s16x8;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
 struct Operand {
     const uint16_t* p;      // plane 0
@@ -38,27 +44,50 @@ template <class T> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// a buffer of `bytes` at p; past them a load delivers zeros
+__device__ __forceinline__ u32x4 buffer_of(const void* p, uint32_t bytes) {
+    const uint64_t b = reinterpret_cast<uint64_t>(p);
+    return {(uint32_t)b, (uint32_t)(b >> 32) & 0xFFFFu, bytes, 0x00020000u};
+}
+
+// 16 bytes a lane from r + offset to LDS at `lds` + 16 lane.  In assembly because the compiler, which cannot tell the stages apart, would wait
+// for every load before the next LDS read: tile_barrier below is the only wait.
+__device__ __forceinline__ void load_to_lds(u32x4 r, uint32_t offset, uint32_t lds) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "s"(lds), "v"(offset), "s"(r) : "memory");
+}
+
 // One operand's tile: TR rows x KT k, NP planes.  PAIR: the tile's rows alternate in blocks of 16 between two K-contiguous operands of
 // the same shape, each with its own pitch (gate and up weights of the same hidden units land in the same wave).
+// The wave loads of a plane (64 x 16 bytes each) go round the waves, so that a wave's loads are a fixed number of LDS rows apart: one offset
+// register serves them all, the rest is scalar.  Rows past the operand's end are past the buffer's.
 template <int TR, int KT, int NP, bool KC, int WAVES, bool PAIR = false> struct TileLoad {
     static constexpr int kPlaneBytes = TR * KT * 2;
     static constexpr int kBytes = kPlaneBytes * NP;
-    static constexpr int kPerPlane = kPlaneBytes / 1024;                 // wave loads of 64 x 16 bytes
-    static constexpr int kLoads = kPerPlane * NP;
-    static constexpr int U = (kLoads + WAVES - 1) / WAVES;
+    static constexpr int kPerPlane = kPlaneBytes / 1024;
+    static constexpr int U = (kPerPlane + WAVES - 1) / WAVES;
     static constexpr int kUnits = KC ? KT / 8 : TR / 8;                  // 16-byte units of an LDS row
-    static_assert(kPlaneBytes % 1024 == 0 && (!PAIR || KC), "whole wave loads");
+    static constexpr int kRowsApart = WAVES * 64 / kUnits;               // LDS rows between a wave's loads
+    static constexpr int kApart = PAIR ? kRowsApart / 2 : kRowsApart;    // operand rows (K-strided: k) between them
+    static_assert(kPlaneBytes % 1024 == 0 && (!PAIR || (KC && kRowsApart % 32 == 0)), "whole wave loads, a wave's of one operand");
+    static_assert(U == 1 || kRowsApart % 16 == 0, "one swizzle for a wave's loads");
 
-    const uint16_t* base[PAIR ? 2 : 1];
+    const uint16_t* base;
     uint64_t plane;
-    uint32_t ld;
-    uint32_t off[U];        // byte offset of the lane's unit from the k-step's base
-    uint32_t kpos[U];       // first k of the lane's unit inside the step
+    uint32_t ld, rows;      // rows of the operand from the tile's first on (K-contiguous)
+    uint32_t off, k_of;     // byte offset of the lane's unit from the k-step's base; its first k (K-contiguous)
 
     // the unit that a row holds at place s, as (row & its swizzle) -- its own inverse
     static __device__ __forceinline__ uint32_t unit_at(uint32_t row, uint32_t s) {
-        if constexpr (KC) return s ^ ((row / (16u / kUnits)) & (kUnits - 1u));
+        if constexpr (KC) return s ^ contiguous_swizzle(row);
         else return s ^ (2u * strided_swizzle(row));
+    }
+    // A 16-byte read takes its 64 lanes in four passes; the first takes lanes 0-3, 12-15 and 20-27, i.e. eight rows of one unit and the other
+    // eight of the unit beside it, the second the rest of that half.  With p = the row in 256-byte periods, units p or p ^ 1 (where p's lanes
+    // read the other unit) are all different.  (The order 0-15, 16-31, ... would want plain p: measured, that costs every read twice its time.)
+    static __device__ __forceinline__ uint32_t contiguous_swizzle(uint32_t row) {
+        const uint32_t p = (row / (16u / kUnits)) & (kUnits - 1u);
+        return p ^ (KT == 32 ? (p ^ (p >> 1)) & 1u : ((p >> 1) ^ (p >> 2)) & 1u);
     }
     static __device__ __forceinline__ uint32_t strided_swizzle(uint32_t k) {
         if constexpr (TR >= 128) return (k & 3u) | ((k >> 1) & 4u);
@@ -67,115 +96,189 @@ template <int TR, int KT, int NP, bool KC, int WAVES, bool PAIR = false> struct 
     }
 
     __device__ __forceinline__ void init(const Operand& a, const Operand& a2, uint32_t row0, uint32_t wave, uint32_t lane) {
-        plane = a.plane;
-        ld = a.ld;
-        base[0] = a.p + (KC ? (uint64_t)row0 * a.ld : (uint64_t)row0);
-        if constexpr (PAIR) base[1] = a2.p + (uint64_t)row0 * a2.ld;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t q = wave * U + u, idx = (q % kPerPlane) * 64u + lane, r = idx / kUnits, c = unit_at(r, idx % kUnits);
-            if constexpr (KC) {
-                const uint32_t row = PAIR ? (r >> 5) * 16u + (r & 15u) : r, pitch = PAIR && ((r >> 4) & 1u) ? a2.ld : a.ld;
-                off[u] = row0 + row < a.ext ? (row * pitch + c * 8u) * 2u : kOutside;
-                kpos[u] = c * 8u;
-            } else {
-                off[u] = row0 + c * 8u < a.ext ? (r * a.ld + c * 8u) * 2u : kOutside;
-                kpos[u] = r;
-            }
+        const uint32_t idx = wave * 64u + lane, r = idx / kUnits, c = unit_at(r, idx % kUnits);
+        const bool second = PAIR && (wave * 64u / kUnits >> 4 & 1u);
+        plane = second ? a2.plane : a.plane;
+        ld = second ? a2.ld : a.ld;
+        base = (second ? a2.p : a.p) + (KC ? (uint64_t)row0 * ld : (uint64_t)row0);
+        if constexpr (KC) {
+            off = ((PAIR ? (r >> 5) * 16u + (r & 15u) : r) * ld + c * 8u) * 2u;
+            k_of = c * 8u;
+            rows = row0 < a.ext ? min(a.ext - row0, (uint32_t)TR) : 0u;
+        } else {
+            off = row0 + c * 8u < a.ext ? (r * ld + c * 8u) * 2u : kOutside;
         }
     }
     // starts the loads of the step that begins at k0 (of K) into `lds`
-    __device__ __forceinline__ void issue(char* lds, uint32_t k0, uint32_t K, uint32_t wave) const {
-        const uint64_t at = KC ? (uint64_t)k0 : (uint64_t)k0 * ld;
-        const bool tail = k0 + KT > K;
+    __device__ __forceinline__ void issue(uint32_t lds, uint32_t k0, uint32_t K, uint32_t wave) const {
+        const uint16_t* b = base + (KC ? (uint64_t)k0 : (uint64_t)k0 * ld);
+        const uint32_t left = KC ? rows : (k0 < K ? min(K - k0, (uint32_t)KT) : 0u);
+        uint32_t o = off;
+        if constexpr (KC) o = k0 + k_of < K ? o : kOutside;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t q = wave * U + u;
-            if (kLoads % WAVES != 0 && q >= (uint32_t)kLoads) break;
-            const uint32_t pl = q / kPerPlane, in_plane = q % kPerPlane;
-            const uint16_t* b = base[0];
-            if constexpr (PAIR) b = (in_plane * 64u / kUnits >> 4) & 1u ? base[1] : base[0];
-            b += (NP > 1 ? pl * plane : 0) + at;
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(b), 0, 0x7FFFFFFF, 0x00020000);
-            uint32_t o = off[u];
-            if (tail) o = k0 + kpos[u] < K ? o : kOutside;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + pl * kPlaneBytes + in_plane * 1024u), 16, o, 0, 0, 0);
+        for (int pl = 0; pl < NP; ++pl) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (kPerPlane % WAVES != 0 && u * WAVES + wave >= (uint32_t)kPerPlane) break;
+                const uint32_t here = left > (uint32_t)(u * kApart) ? (left - u * kApart) * ld * 2u : 0u;
+                load_to_lds(buffer_of(b + pl * plane + (uint64_t)(u * kApart) * ld, here), o, lds + pl * kPlaneBytes + (u * WAVES + wave) * 1024u);
+            }
         }
     }
-    // operand of sixteen tile rows from `row16` on (a multiple of 16), k block kk of 32
-    static __device__ __forceinline__ s16x8 fragment(const char* lds, int pl, uint32_t row16, int kk, uint32_t lane) {
+    // operand of sixteen tile rows from `row16` on (a multiple of 16), k block kk of 32; lds: the tile's LDS address.  (The K-strided form adds
+    // the tile's address before the exclusive or: that way the addresses of a step are formed in the step and take no registers across it.)
+    static __device__ __forceinline__ s16x8 fragment(uint32_t lds, int pl, uint32_t row16, int kk, uint32_t lane) {
         const uint32_t g = lane >> 4, i = lane & 15u;
         if constexpr (KC) {
-            const uint32_t c = (uint32_t)kk * 4u + g;
-            return *reinterpret_cast<const s16x8*>(lds + pl * kPlaneBytes + (row16 + i) * (KT * 2u) + unit_at(i, c) * 16u);
+            const uint32_t at = lds + i * (KT * 2u) + unit_at(i, (uint32_t)kk * 4u + g) * 16u;
+            return *(const lds_s16x8*)(at + pl * kPlaneBytes + row16 * (KT * 2u));
         } else {
             const uint32_t k = 8u * g + (i >> 2);            // (kk * 32 and + 4 leave the swizzle as it is)
-            const uint32_t at = (k * TR * 2u + strided_swizzle(k) * 32u + (i & 3u) * 8u) ^ (row16 * 2u);
-            const char* p = lds + pl * kPlaneBytes + kk * 32 * TR * 2 + at;
+            const uint32_t at = (lds + k * TR * 2u + strided_swizzle(k) * 32u + (i & 3u) * 8u) ^ (row16 * 2u & 255u);
+            const uint32_t p = at + (row16 * 2u & ~255u) + pl * kPlaneBytes + kk * 32 * TR * 2;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * TR * 2));
             return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
 };
 
-// every load of this wave has landed, every LDS read of it is done, and so for the whole workgroup
-__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// At most N of this wave's LDS-direct loads are still in flight, every LDS read of it is done, and so for the whole workgroup
+template <int N> __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
 // A workgroup's K loop over one pair of operands: acc[mi][ni] += A rows x B rows.  Wave (wm, wn) of WM x WN owns 16 MI x 16 NI of the tile.
-// Two LDS stages: the loads of a step run under the products of the step before.
-template <class T, int NP, int KT, int TM, int TN, int WM, int WN, bool AKC, bool BKC, bool PAIR> struct Product {
+// Memory -> LDS: S stages of KT, S steps ahead; LDS -> registers: 32 k ahead, so that the reads run under the products of the 32 before
+// (the waves of a workgroup pass the barrier together: without this they would all read, then all multiply).
+//   barrier t: step t + 1 has landed for everyone, and everyone has the last of step t in registers, so its stage is free for step t + S
+// Steps past the end are loads of zeros: the number in flight is the same at every wait.
+template <class T, int NP, int TM, int TN, int WM, int WN, bool AKC, bool BKC, bool PAIR> struct Product {
+    static constexpr int KT = NP == 1 ? 64 : 32;
     static constexpr int WAVES = WM * WN, MI = TM / WM / 16, NI = TN / WN / 16;
     using LA = TileLoad<TM, KT, NP, AKC, WAVES>;
     using LB = TileLoad<TN, KT, NP, BKC, WAVES, PAIR>;
     static constexpr int kStage = LA::kBytes + LB::kBytes;
 
-    template <int ACC> static __device__ __forceinline__ void compute(const char* lds, uint32_t wm, uint32_t wn, uint32_t lane, f32x4 (&acc)[MI][ACC], int at) {
+    struct Fragments {
+        s16x8 a[NP][MI], b[NP][NI];
+    };
+    static __device__ __forceinline__ void read_a(uint32_t lds, int kk, int p, uint32_t wm, uint32_t lane, s16x8 (&a)[MI]) {
 #pragma unroll
-        for (int kk = 0; kk < KT / 32; ++kk) {
-            s16x8 fa[NP][MI], fb[NP][NI];
+        for (int mi = 0; mi < MI; ++mi) a[mi] = LA::fragment(lds, p, (wm * MI + mi) * 16u, kk, lane);
+    }
+    static __device__ __forceinline__ void read_b(uint32_t lds, int kk, int p, uint32_t wn, uint32_t lane, s16x8 (&b)[NI]) {
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
+        for (int ni = 0; ni < NI; ++ni) b[ni] = LB::fragment(lds + LA::kBytes, p, (wn * NI + ni) * 16u, kk, lane);
+    }
+    static __device__ __forceinline__ void read(uint32_t lds, int kk, uint32_t wm, uint32_t wn, uint32_t lane, Fragments& f) {
 #pragma unroll
-                for (int ni = 0; ni < NI; ++ni) fb[p][ni] = LB::fragment(lds + LA::kBytes, p, (wn * NI + ni) * 16u, kk, lane);
-#pragma unroll
-                for (int mi = 0; mi < MI; ++mi) fa[p][mi] = LA::fragment(lds, p, (wm * MI + mi) * 16u, kk, lane);
-            }
-#pragma unroll
-            for (int pa = 0; pa < NP; ++pa)
-#pragma unroll
-                for (int pb = 0; pb < NP; ++pb) {
-                    if (pa + pb > 2) continue;
-#pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                        for (int ni = 0; ni < NI; ++ni) acc[mi][at + ni] = mfma16<T>(fb[pb][ni], fa[pa][mi], acc[mi][at + ni]);
-                }
+        for (int p = 0; p < NP; ++p) {
+            read_b(lds, kk, p, wn, lane, f.b[p]);
+            read_a(lds, kk, p, wm, lane, f.a[p]);
         }
     }
-    // [k_from, k_to) of the reduction; acc's columns at .. at + NI - 1.  lds0 / lds1: the two stages.  Leaves with every LDS read done.
-    template <int ACC> static __device__ __forceinline__ void run(const Operand& A, const Operand& B, const Operand& B2, uint32_t row0, uint32_t col0, uint32_t k_from, uint32_t k_to, char* lds0, char* lds1,
-                                                                  f32x4 (&acc)[MI][ACC], int at) {
-        const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    template <int ACC> static __device__ __forceinline__ void multiply(const s16x8 (&a)[MI], const s16x8 (&b)[NI], f32x4 (&acc)[MI][ACC], int at) {
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) acc[mi][at + ni] = mfma16<T>(b[ni], a[mi], acc[mi][at + ni]);
+    }
+    // the products of the step in `f`; `next`: the step behind it, read from `lds`
+    template <int ACC> static __device__ __forceinline__ void step(uint32_t lds, int kk, uint32_t wm, uint32_t wn, uint32_t lane, Fragments& f, Fragments& next, f32x4 (&acc)[MI][ACC], int at) {
+        if constexpr (NP == 1) {
+            read(lds, kk, wm, wn, lane, next);
+            multiply(f.a[0], f.b[0], acc, at);
+        } else {
+            // the small products first; a term's registers take the next step's as soon as its last product is out
+            multiply(f.a[0], f.b[2], acc, at);
+            read_b(lds, kk, 2, wn, lane, next.b[2]);
+            multiply(f.a[2], f.b[0], acc, at);
+            read_a(lds, kk, 2, wm, lane, next.a[2]);
+            multiply(f.a[1], f.b[1], acc, at);
+            multiply(f.a[0], f.b[1], acc, at);
+            read_b(lds, kk, 1, wn, lane, next.b[1]);
+            multiply(f.a[1], f.b[0], acc, at);
+            read_a(lds, kk, 1, wm, lane, next.a[1]);
+            read_a(lds, kk, 0, wm, lane, next.a[0]);
+            read_b(lds, kk, 0, wn, lane, next.b[0]);
+            multiply(f.a[0], f.b[0], acc, at);
+        }
+    }
+    // The loads' side of the pipeline: where the next step comes from.
+    struct Source {
         LA la;
         LB lb;
-        la.init(A, A, row0, wave, lane);
-        lb.init(B, B2, col0, wave, lane);
-        auto issue = [&](char* lds, uint32_t k0) {
-            la.issue(lds, k0, k_to, wave);
-            lb.issue(lds + LA::kBytes, k0, k_to, wave);
-        };
-        if (k_from < k_to) issue(lds0, k_from);
-        for (uint32_t k0 = k_from; k0 < k_to; k0 += 2 * KT) {
-            tile_barrier();
-            if (k0 + KT < k_to) issue(lds1, k0 + KT);
-            compute(lds0, wm, wn, lane, acc, at);
-            if (k0 + KT >= k_to) break;
-            tile_barrier();
-            if (k0 + 2 * KT < k_to) issue(lds0, k0 + 2 * KT);
-            compute(lds1, wm, wn, lane, acc, at);
+        uint32_t ahead, to;
+        __device__ __forceinline__ void init(const Operand& A, const Operand& B, const Operand& B2, uint32_t row0, uint32_t col0, uint32_t k_from, uint32_t k_to) {
+            const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            la.init(A, A, row0, wave, lane);
+            lb.init(B, B2, col0, wave, lane);
+            ahead = k_from;
+            to = k_to;
         }
-        tile_barrier();
+        __device__ __forceinline__ void issue(uint32_t lds) {
+            const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            la.issue(lds, ahead, to, wave);
+            lb.issue(lds + LA::kBytes, ahead, to, wave);
+            ahead += KT;
+        }
+    };
+    // steps of a reduction of length k: at least the two that are under way before it starts, an even number where the registers' roles alternate
+    static __device__ __forceinline__ uint32_t steps(uint32_t k) {
+        const uint32_t n = (k + KT - 1) / KT;
+        return KT == 32 ? (n < 2 ? 2u : (n + 1u) & ~1u) : (n < 2 ? 2u : n);
     }
+    // acc's columns at .. at + NI - 1 += the n steps whose first two are under way into the stages `stage`, stage_bytes - `stage` (offsets from
+    // lds) from `src`.  `turn` is called when all loads of these steps are out; issue_next(lds) then starts the steps of what comes next: two of
+    // them are under way on return, the first into `stage`.
+    // relaxed: exactly STORES memory operations were issued behind the first two steps' loads (the tile before's results); they may stay
+    // in flight while those steps are waited for -- operations complete in order, so "all but the last STORES" are the loads.
+    template <int STORES, int ACC, class Turn, class Issue>
+    static __device__ __forceinline__ void run(uint32_t lds, uint32_t stage_bytes, uint32_t& stage, Source& src, uint32_t n, bool relaxed, f32x4 (&acc)[MI][ACC], int at, Turn turn, Issue issue_next) {
+        const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+        Fragments f[2];
+        auto barrier = [&](bool first) {
+            if (STORES > 0 && first && relaxed) tile_barrier<STORES>();
+            else tile_barrier<0>();
+        };
+        barrier(true);
+        read(lds + stage, 0, wm, wn, lane, f[0]);
+        auto one = [&](Fragments& now, Fragments& then, bool first, bool last) {
+            const uint32_t other = stage_bytes - stage;
+            if constexpr (KT == 64) step(lds + stage, 1, wm, wn, lane, now, then, acc, at);
+            barrier(first);
+            if (!last) src.issue(lds + stage); else issue_next(lds + stage);
+            if constexpr (KT == 64) step(lds + other, 0, wm, wn, lane, then, now, acc, at);
+            else step(lds + other, 0, wm, wn, lane, now, then, acc, at);
+            stage = other;
+        };
+        if constexpr (KT == 64) {
+            for (uint32_t s = 0; s + 2 < n; ++s) one(f[0], f[1], s == 0, false);
+            turn();
+            one(f[0], f[1], n == 2, true);
+            one(f[0], f[1], false, true);
+        } else {
+            for (uint32_t s = 0; s + 2 < n; s += 2) {
+                one(f[0], f[1], s == 0, false);
+                one(f[1], f[0], false, false);
+            }
+            turn();
+            one(f[0], f[1], n == 2, true);
+            one(f[1], f[0], false, true);
+        }
+    }
+};
+
+// A workgroup's share of the tiles.  Workgroups go to the eight XCDs in turn: each XCD gets a run of adjacent tiles, column tiles first, so that
+// the rows of a run and the weights stay in its own L2; its workgroups walk the run side by side.
+struct TileWalk {
+    uint32_t now, end, by;
+    __device__ __forceinline__ TileWalk(uint32_t tiles) {
+        const uint32_t each = (tiles + 7u) / 8u, first = (blockIdx.x & 7u) * each;
+        now = first + (blockIdx.x >> 3);
+        end = min(first + each, tiles);
+        by = gridDim.x >> 3;
+    }
+    __device__ __forceinline__ bool valid() const { return now < end; }
+    __device__ __forceinline__ bool more() const { return now + by < end; }
 };
 
 // an fp32 number as its three bf16 terms (exact: 8 + 8 + 8 bits); the first is truncated where rounding it would overflow
@@ -208,6 +311,36 @@ template <class T, int NP> __device__ __forceinline__ void store_planes(uint16_t
     }
 }
 
+// one memory operation, dropped by the lanes whose offset is past the `bytes` at p
+__device__ __forceinline__ void store_to_buffer(u32x4 v, void* p, uint32_t bytes, uint32_t offset) {
+    __builtin_amdgcn_raw_buffer_store_b128(v, __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00020000), offset, 0, 0);
+}
+
+// Sixteen-bit results on their way out.  A wave holds, of each row of a 16-row block, four adjacent columns in each lane group: stored like
+// that a row is written 32 bytes at a time.  Through 2 KiB of LDS of its own the wave turns 1024 / COLS rows of COLS columns into whole rows.
+template <int COLS> struct RowStore {
+    static constexpr int kRows = 1024 / COLS, kUnits = COLS / 8, kBytes = 2048;
+    typedef __attribute__((address_space(3))) s16x4 lds_half;
+    // columns col .. col + 3 of row `row` of the block
+    static __device__ __forceinline__ void put(uint32_t lds, uint32_t row, uint32_t col, s16x4 v) {
+        const uint32_t unit = (col >> 3) ^ (row & (kUnits - 1u));
+        *(lds_half*)(lds + row * (COLS * 2u) + unit * 16u + (col & 4u) * 2u) = v;
+    }
+    static constexpr int kStores = 2;
+    // the block's rows to p (its first row, `rows` of them there) from column col0 on (`cols` of them there): 16-byte aligned, whole units.
+    // Always kStores memory operations.
+    static __device__ __forceinline__ void flush(uint32_t lds, uint16_t* p, uint32_t ld, uint32_t rows, uint32_t col0, uint32_t cols) {
+        const uint32_t lane = threadIdx.x & 63u;
+        const uint32_t bytes = min(rows, (uint32_t)kRows) * ld * 2u;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t idx = j * 64u + lane, row = idx / kUnits, unit = idx % kUnits, col = col0 + unit * 8u;
+            const u32x4 v = *(const lds_u32x4*)(lds + row * (COLS * 2u) + (unit ^ (row & (kUnits - 1u))) * 16u);
+            store_to_buffer(v, p, bytes, col < cols ? (row * ld + col) * 2u : kOutside);
+        }
+    }
+};
+
 // up to four adjacent results of a row of an output of any alignment: `left` columns of it remain
 template <class E> __device__ __forceinline__ void store_row4(E* p, int64_t left, const float (&v)[4]) {
     if (left >= 4) {
@@ -221,5 +354,97 @@ template <class E> __device__ __forceinline__ void store_row4(E* p, int64_t left
             if (r < left) p[r] = from_f32<E>(v[r]);
     }
 }
+
+template <class T> __device__ __forceinline__ s16x4 pack4(const float (&v)[4]) {
+    Pack<T, 4> o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o.v[r] = from_f32<T>(v[r]);
+    return __builtin_bit_cast(s16x4, o);
+}
+
+// A wave's results acc[MI][NI], its rows from row0 and columns from col0 on, to out [rows][cols] with pitch ld.  aligned: whole 16-byte units
+// everywhere, and then exactly kCount memory operations.  scratch: 2 KiB of LDS (16-bit results).
+template <class E, int MI, int NI> struct ResultStore {
+    static constexpr bool kWide = sizeof(E) == 4;
+    static constexpr int kCount = kWide ? MI * NI : MI * 16 / RowStore<NI * 16>::kRows * 2;
+    static __device__ __forceinline__ void store(uint32_t scratch, const f32x4 (&acc)[MI][NI], E* out, int64_t ld, uint32_t rows, uint32_t cols, uint32_t row0, uint32_t col0, bool aligned) {
+        const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, g = lane >> 4;
+        if (!aligned) {
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi) {
+                const uint32_t m = row0 + mi * 16u + i;
+                if (m >= rows) continue;
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni) {
+                    const uint32_t n = col0 + ni * 16u + 4u * g;
+                    const float v[4] = {acc[mi][ni][0], acc[mi][ni][1], acc[mi][ni][2], acc[mi][ni][3]};
+                    store_row4(out + (int64_t)m * ld + n, (int64_t)cols - n, v);
+                }
+            }
+            return;
+        }
+        if constexpr (kWide) {
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi) {
+                const uint32_t m0 = row0 + mi * 16u, left = m0 < rows ? min(rows - m0, 16u) : 0u;
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni) {
+                    const uint32_t n = col0 + ni * 16u + 4u * g;
+                    store_to_buffer(__builtin_bit_cast(u32x4, acc[mi][ni]), out + (int64_t)m0 * ld, left * (uint32_t)ld * 4u, n < cols ? (i * (uint32_t)ld + n) * 4u : kOutside);
+                }
+            }
+        } else {
+            using W = RowStore<NI * 16>;
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi) {
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni) {
+                    const float v[4] = {acc[mi][ni][0], acc[mi][ni][1], acc[mi][ni][2], acc[mi][ni][3]};
+                    W::put(scratch, mi * 16u % W::kRows + i, ni * 16u + 4u * g, pack4<E>(v));
+                }
+                if ((mi + 1) * 16 % W::kRows == 0) {
+                    const uint32_t m0 = row0 + (mi + 1) * 16u - W::kRows;
+                    W::flush(scratch, reinterpret_cast<uint16_t*>(out + (int64_t)m0 * ld), (uint32_t)ld, m0 < rows ? rows - m0 : 0u, col0, cols);
+                }
+            }
+        }
+    }
+};
+
+// Rows of 32-bit values on their way to an operand of the next product: COLS columns of kRows rows, as NP planes
+template <class T, int NP, int COLS> struct PlaneStore {
+    using W = RowStore<COLS>;
+    static constexpr int kBlocks = W::kRows / 16, kCount = 2 * NP;       // 16-row blocks, memory operations
+    // v[block][nj][r]: column 16 nj + 4 (lane / 16) + r of row 16 block + lane % 16
+    static __device__ __forceinline__ void store(uint32_t scratch, const float (&v)[kBlocks][COLS / 16][4], uint16_t* out, uint64_t plane, uint32_t ld, uint32_t rows, uint32_t row0, uint32_t col0, uint32_t cols) {
+        const uint32_t lane = threadIdx.x & 63u;
+        float rest[kBlocks][COLS / 16][4];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int j = 0; j < COLS / 16; ++j) {
+                    s16x4 o;
+                    if constexpr (NP == 1) {
+                        o = pack4<T>(v[b][j]);
+                    } else {
+                        // (the terms one after the other, as split3 makes them)
+                        Pack<__bf16, 4> t;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float x = p == 0 ? v[b][j][r] : rest[b][j][r];
+                            t.v[r] = (__bf16)x;
+                            if (p == 0 && __builtin_isinf((float)t.v[r])) t.v[r] = __builtin_bit_cast(__bf16, (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16));
+                            rest[b][j][r] = x - (float)t.v[r];
+                        }
+                        o = __builtin_bit_cast(s16x4, t);
+                    }
+                    W::put(scratch, b * 16u + (lane & 15u), j * 16u + 4u * (lane >> 4), o);
+                }
+            W::flush(scratch, out + p * plane + (uint64_t)row0 * ld, ld, row0 < rows ? rows - row0 : 0u, col0, cols);
+        }
+    }
+};
 
 }  // namespace envidr
