@@ -17,8 +17,7 @@ def _forward(gate, value, rays, state, code, blend, keep):
     T, C = gate.shape
     N = rays.shape[0]
     h = torch.empty(T, C, dtype=gate.dtype, device=gate.device)
-    # (an id that no ray names keeps its state)
-    last = torch.zeros(N, C, dtype=torch.float32, device=gate.device) if state is None else state.clone()
+    last = torch.empty(N, C, dtype=torch.float32, device=gate.device)
     saved = torch.empty(lib.envidr_ray_recurrence_saved_floats(T, N, C), dtype=torch.float32, device=gate.device) if keep else None
     with _bind.on_device(gate) as stream:
         ws, n = _workspace(lib, T, N, C, gate.device)
@@ -46,7 +45,7 @@ class _RayRecurrence(torch.autograd.Function):
         dh = dh.contiguous()
         dlast = dlast.contiguous()
         dgate, dvalue = torch.empty_like(gate), torch.empty_like(value)
-        dstate = dlast.clone() if ctx.needs_input_grad[2] else None          # (an id that no ray names: last was its state)
+        dstate = torch.empty_like(dlast) if ctx.needs_input_grad[2] else None
         with _bind.on_device(gate) as stream:
             ws, n = _workspace(lib, T, N, C, gate.device)
             _bind.check(lib.envidr_ray_recurrence_backward(dh.data_ptr(), dlast.data_ptr(), gate.data_ptr(), value.data_ptr(), rays.data_ptr(),

@@ -58,8 +58,8 @@ int envidr_gated_mlp_backward(const void* dy, int64_t lddy, const void* x, int64
  *   gate, value, h [T, C]; rays int32 [N, 3] = (id, offset, count) as envidr_march_rays_train writes them: rows offset .. offset + count - 1
  *   are the samples of ray `id`, front to back.  Rays may come in any order and leave rows between and behind them; no two may share a
  *   row.  A ray with count <= 0, offset < 0 or offset + count > T has no rows (the compositors' rule).
- *   state fp32 [N, C] or NULL (zeros): h before the first sample, indexed by id; last fp32 [N, C]: h after the last one (the state of a ray
- *   without rows), written for every id in 0 .. N-1 that `rays` names (an id outside is treated as a ray without state).
+ *   state fp32 [N, C] or NULL (zeros): h before the first sample, indexed by id; last fp32 [N, C]: h after the last one.  The id of a ray
+ *   without rows, and an id that no ray names, keep their state; a ray with an id outside 0 .. N-1 starts from zeros and leaves none.
  *   Rows that belong to no ray: h, dgate and dvalue are zero there.
  *   saved: fp32 [envidr_ray_recurrence_saved_floats(T, N, C)] or NULL; written by the forward pass and read by the backward one of the
  *   same inputs.

@@ -99,7 +99,7 @@ def test_ray_recurrence_refuses_what_it_cannot_take():
     _refused(backward(rays=None), b"null pointer")
     _refused(backward(n=0), b"workspace")
     # states, marks and owners: in proportion to the rows
-    assert lib.envidr_ray_recurrence_saved_floats(1 << 20, 4, 64) < (1 << 20) * (64 // 16 + 2)
+    assert lib.envidr_ray_recurrence_saved_floats(1 << 20, 4, 64) < (1 << 20) * (64 // 8 + 2)
 
 
 def test_dropout_refuses_what_it_cannot_take():
