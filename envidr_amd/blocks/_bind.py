@@ -61,16 +61,17 @@ def same_kind(name: str, first: torch.Tensor, **others: torch.Tensor | None) -> 
 class on_device:
     """The tensor's device as the current one for the launches inside (a no-op when it is already), and its current stream."""
 
+    __slots__ = ("index", "before")
+
     def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
-        self.before = None
+        self.index = t.get_device()
 
     def __enter__(self) -> int:
-        if torch.cuda.current_device() != self.index:
-            self.before = torch.cuda.current_device()
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.index)          # (what torch.cuda.current_stream().cuda_stream is, without the object)
 
     def __exit__(self, *exc) -> None:
-        if self.before is not None:
+        if self.before != self.index:
             torch.cuda.set_device(self.before)

@@ -1,6 +1,8 @@
 """The gated feed-forward block (envidr_gated_mlp_*, csrc/gated_mlp.hip):  y = (act(x Wg^T) * (x Wu^T)) Wd^T  and its gradients."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -19,17 +21,18 @@ def _sizes(x, wg, wd):
     return x.shape[0], x.shape[1], wg.shape[0], wd.shape[0]
 
 
-def _workspace(lib, M, D, F, O, code, backward, device):
-    n = lib.envidr_gated_mlp_workspace_bytes(M, D, F, O, code, backward)
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=device), n
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(M, D, F, O, code, backward):
+    return max(_bind.lib().envidr_gated_mlp_workspace_bytes(M, D, F, O, code, backward), 16)
 
 
 def _forward(x, wg, wu, wd, code, act):
     lib = _bind.lib()
     M, D, F, O = _sizes(x, wg, wd)
-    y = torch.empty(M, O, dtype=x.dtype, device=x.device)
+    n = _workspace_bytes(M, D, F, O, code, 0)
+    y = torch.empty((M, O), dtype=x.dtype, device=x.device)
     with _bind.on_device(x) as stream:
-        ws, n = _workspace(lib, M, D, F, O, code, 0, x.device)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
         _bind.check(lib.envidr_gated_mlp_forward(x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), wd.data_ptr(), wd.stride(0),
                                                  M, D, F, O, code, act, y.data_ptr(), O, ws.data_ptr(), n, stream), "envidr_gated_mlp_forward")
     return y
@@ -51,11 +54,11 @@ class _GatedMlp(torch.autograd.Function):
         lib = _bind.lib()
         M, D, F, O = _sizes(x, wg, wd)
         dy = _rows(dy)
-        new = lambda want, *shape: torch.empty(*shape, dtype=x.dtype, device=x.device) if want else None  # noqa: E731
-        grads = [new(want, *shape) for want, shape in zip(ctx.needs_input_grad, ((M, D), (F, D), (F, D), (O, F)))]
+        n = _workspace_bytes(M, D, F, O, ctx.code, 1)
+        grads = [torch.empty(shape, dtype=x.dtype, device=x.device) if want else None for want, shape in zip(ctx.needs_input_grad, ((M, D), (F, D), (F, D), (O, F)))]
         at = [None if g is None else g.data_ptr() for g in grads]
         with _bind.on_device(x) as stream:
-            ws, n = _workspace(lib, M, D, F, O, ctx.code, 1, x.device)
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
             _bind.check(lib.envidr_gated_mlp_backward(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0),
                                                       wd.data_ptr(), wd.stride(0), M, D, F, O, ctx.code, ctx.act, at[0], D, at[1], at[2], at[3],
                                                       ws.data_ptr(), n, stream), "envidr_gated_mlp_backward")

@@ -1,28 +1,34 @@
 """A gated linear recurrence along the samples of packed rays (envidr_ray_recurrence_*, csrc/ray_recurrence.hip)."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
 from . import _bind
 
 
-def _workspace(lib, T, N, C, device):
-    n = lib.envidr_ray_recurrence_workspace_bytes(T, N, C)
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=device), n
+@functools.lru_cache(maxsize=256)
+def _sizes(T, N, C):
+    """bytes of the workspace, floats of what the forward pass leaves for the backward one"""
+    lib = _bind.lib()
+    return max(lib.envidr_ray_recurrence_workspace_bytes(T, N, C), 16), lib.envidr_ray_recurrence_saved_floats(T, N, C)
 
 
 def _forward(gate, value, rays, state, code, blend, keep):
     lib = _bind.lib()
     T, C = gate.shape
     N = rays.shape[0]
-    h = torch.empty(T, C, dtype=gate.dtype, device=gate.device)
-    last = torch.empty(N, C, dtype=torch.float32, device=gate.device)
-    saved = torch.empty(lib.envidr_ray_recurrence_saved_floats(T, N, C), dtype=torch.float32, device=gate.device) if keep else None
+    device = gate.device
+    n, n_saved = _sizes(T, N, C)
+    h = torch.empty((T, C), dtype=gate.dtype, device=device)
+    last = torch.empty((N, C), dtype=torch.float32, device=device)
+    saved = torch.empty(n_saved, dtype=torch.float32, device=device) if keep else None
     with _bind.on_device(gate) as stream:
-        ws, n = _workspace(lib, T, N, C, gate.device)
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
         _bind.check(lib.envidr_ray_recurrence_forward(gate.data_ptr(), value.data_ptr(), rays.data_ptr(), None if state is None else state.data_ptr(), T, N, C, code, blend,
-                                                      h.data_ptr(), last.data_ptr(), None if saved is None else saved.data_ptr(), ws.data_ptr(), n, stream),
+                                                      h.data_ptr(), last.data_ptr(), saved.data_ptr() if keep else None, ws.data_ptr(), n, stream),
                     "envidr_ray_recurrence_forward")
     return h, last, saved
 
@@ -33,6 +39,7 @@ class _RayRecurrence(torch.autograd.Function):
         h, last, saved = _forward(gate, value, rays, state, code, blend, True)
         ctx.save_for_backward(gate, value, state, rays, saved)
         ctx.code, ctx.blend = code, blend
+        ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
@@ -42,13 +49,16 @@ class _RayRecurrence(torch.autograd.Function):
         lib = _bind.lib()
         T, C = gate.shape
         N = rays.shape[0]
-        dh = dh.contiguous()
-        dlast = dlast.contiguous()
-        dgate, dvalue = torch.empty_like(gate), torch.empty_like(value)
-        dstate = torch.empty_like(dlast) if ctx.needs_input_grad[2] else None
+        device = gate.device
+        n = _sizes(T, N, C)[0]
+        dh = torch.zeros((T, C), dtype=gate.dtype, device=device) if dh is None else dh.contiguous()
+        if dlast is not None:
+            dlast = dlast.contiguous()
+        dgate, dvalue = (torch.empty((T, C), dtype=gate.dtype, device=device) for _ in range(2))
+        dstate = torch.empty((N, C), dtype=torch.float32, device=device) if ctx.needs_input_grad[2] else None
         with _bind.on_device(gate) as stream:
-            ws, n = _workspace(lib, T, N, C, gate.device)
-            _bind.check(lib.envidr_ray_recurrence_backward(dh.data_ptr(), dlast.data_ptr(), gate.data_ptr(), value.data_ptr(), rays.data_ptr(),
+            ws = torch.empty(n, dtype=torch.uint8, device=device)
+            _bind.check(lib.envidr_ray_recurrence_backward(dh.data_ptr(), None if dlast is None else dlast.data_ptr(), gate.data_ptr(), value.data_ptr(), rays.data_ptr(),
                                                            None if state is None else state.data_ptr(), saved.data_ptr(), T, N, C, ctx.code, ctx.blend,
                                                            dgate.data_ptr(), dvalue.data_ptr(), None if dstate is None else dstate.data_ptr(), ws.data_ptr(), n, stream),
                         "envidr_ray_recurrence_backward")

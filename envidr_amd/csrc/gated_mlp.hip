@@ -162,6 +162,8 @@ struct ProductArgs {
     int64_t ld;
     uint32_t M, N, col_tiles, tiles;
     bool aligned;
+    uint32_t splits, per_split;     // splits > 0: each phase's reduction is cut into that many, and every part is a tile of its own whose sums
+    float* part;                    // go to part [phases * splits][M][N]
 };
 
 // rows x columns results of type E: BKC: b K-contiguous (y = h Wd^T), else K-strided (dx = dg Wg + du Wu)
@@ -170,24 +172,41 @@ template <class E, class T, int NP, int TM, int TN, int WM, int WN, bool BKC> __
     using Out = ResultStore<E, P::MI, P::NI>;
     __shared__ __attribute__((aligned(1024))) char lds_all[2 * P::kStage + (Out::kWide ? 0 : WM * WN * 2048)];
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)lds_all, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), scratch = lds + 2 * P::kStage + wave * 2048u;
-    TileWalk walk(a.tiles);
+    TileWalk walk(a.tiles * (a.splits ? a.splits * a.phases : 1u));
     if (!walk.valid()) return;
     typename P::Source src;
-    const uint32_t n = P::steps(a.K);
-    auto aim = [&](uint32_t t, uint32_t p) { src.init(p ? a.a[1] : a.a[0], p ? a.b[1] : a.b[0], a.b[0], t / a.col_tiles * TM, t % a.col_tiles * TN, 0, a.K); };
-    aim(walk.now, 0);
+    struct Spot { uint32_t part, row0, col0, phase, from, to; };
+    auto spot = [&](uint32_t i, uint32_t p) {
+        Spot s;
+        const uint32_t t = i % a.tiles;
+        s.part = i / a.tiles;
+        s.row0 = t / a.col_tiles * TM;
+        s.col0 = t % a.col_tiles * TN;
+        s.phase = a.splits ? s.part / a.splits : p;
+        s.from = a.splits ? min(s.part % a.splits * a.per_split, a.K) : 0u;
+        s.to = a.splits ? min(s.from + a.per_split, a.K) : a.K;
+        return s;
+    };
+    auto aim = [&](const Spot& s) { src.init(s.phase ? a.a[1] : a.a[0], s.phase ? a.b[1] : a.b[0], a.b[0], s.row0, s.col0, s.from, s.to); };
+    const uint32_t runs = a.splits ? 1u : a.phases;             // one after the other into the same sums
+    Spot now = spot(walk.now, 0), next = now;
+    aim(now);
     src.issue(lds);
     src.issue(lds + P::kStage);
     uint32_t stage = 0;
     for (bool fresh = true; walk.valid(); walk.now += walk.by, fresh = false) {
         const bool more = walk.more();
         f32x4 acc[P::MI][P::NI] = {};
-        for (uint32_t p = 0; p < a.phases; ++p) {
-            const bool goes_on = more || p + 1 < a.phases;
-            P::template run<Out::kCount>(lds, P::kStage, stage, src, n, !fresh && a.aligned && p == 0, acc, 0,
-                                         [&] { if (p + 1 < a.phases) aim(walk.now, p + 1); else if (more) aim(walk.now + walk.by, 0); }, [&](uint32_t to) { if (goes_on) src.issue(to); });
+        for (uint32_t p = 0; p < runs; ++p) {
+            const bool goes_on = more || p + 1 < runs;
+            P::template run<Out::kCount>(lds, P::kStage, stage, src, P::steps(now.to - now.from), !fresh && a.aligned && p == 0 && !a.splits, acc, 0,
+                                         [&] { if (goes_on) { next = p + 1 < runs ? spot(walk.now, p + 1) : spot(walk.now + walk.by, 0); aim(next); } }, [&](uint32_t to) { if (goes_on) src.issue(to); });
+            if (p + 1 < runs) now = next;
         }
-        Out::store(scratch, acc, static_cast<E*>(a.out), a.ld, a.M, a.N, walk.now / a.col_tiles * TM + wave / WN * (P::MI * 16u), walk.now % a.col_tiles * TN + wave % WN * (P::NI * 16u), a.aligned);
+        const uint32_t row0 = now.row0 + wave / WN * (P::MI * 16u), col0 = now.col0 + wave % WN * (P::NI * 16u);
+        if (a.splits) ResultStore<float, P::MI, P::NI>::store(scratch, acc, a.part + (uint64_t)now.part * a.M * a.N, a.N, a.M, a.N, row0, col0, a.N % 4u == 0);
+        else Out::store(scratch, acc, static_cast<E*>(a.out), a.ld, a.M, a.N, row0, col0, a.aligned);
+        now = next;
     }
 }
 
@@ -261,10 +280,11 @@ template <class E, class T, int NP, int TM, int TN, int WM, int WN> __global__ v
 }
 
 struct SumJob {
-    const float* part;
+    const float* part;              // [splits][n / cols][cols]
     void* out;
     uint64_t n;
-    uint32_t first_block;
+    uint32_t first_block, cols;
+    int64_t ld;                     // of out
 };
 struct SumArgs {
     SumJob job[3];
@@ -278,7 +298,7 @@ template <class E> __global__ void __launch_bounds__(kBlock) k_sum_splits(SumArg
     if (i >= s.n) return;
     float v = 0;
     for (uint32_t k = 0; k < a.splits; ++k) v += s.part[k * s.n + i];
-    static_cast<E*>(s.out)[i] = from_f32<E>(v);
+    static_cast<E*>(s.out)[(int64_t)(i / s.cols) * s.ld + (int64_t)(i % s.cols)] = from_f32<E>(v);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------------------------
@@ -360,6 +380,8 @@ struct Plan {
     uint32_t np, Dp, Fp, Op, chunk;
     uint32_t splits, per_split;
     bool large_grads;
+    uint32_t product_splits, product_per_split;     // of y's reduction, or of either of dx's
+    uint64_t product_part;
     uint64_t x, dy, wg, wu, wd, h, dg, du, part, bytes;
 };
 
@@ -378,6 +400,19 @@ uint64_t grad_tiles(uint32_t D, uint32_t F, uint32_t O, TileSize t) { return 2 *
 uint32_t grid_of(uint64_t tiles, uint32_t per_cu) {
     const uint64_t all = (tiles + 7) / 8 * 8, most = (uint64_t)kCus * per_cu;
     return (uint32_t)(all < most ? all : most);
+}
+
+// Few tiles and a long reduction (a small batch through a wide layer): a step of the reduction costs a workgroup about 0.7 us of latency however
+// few workgroups there are, so each reduction is cut until the tiles' parts fill the chip, in parts of four steps at least.  From twelve
+// steps on that gains more than the launch that adds the parts up costs (500 x 1000 outputs over 4000: 44 -> 15 us).
+uint32_t product_splits(uint64_t rows, uint64_t cols, uint32_t k, uint32_t phases, uint32_t np) {
+    if (large_product(rows, cols, np)) return 0;
+    const uint32_t steps = ceil_div(k, np == 1 ? 64u : 32u);
+    const uint64_t tiles = tiles_of(rows, cols, product_tile(np, false)) * phases, slots = kCus * (np == 1 ? 2u : 1u);
+    if (tiles * 2 > slots || steps * phases < 12u) return 0;
+    const uint64_t fill = slots / tiles, can = steps / 4u ? steps / 4u : 1u;
+    const uint64_t splits = fill < can ? fill : can;
+    return splits * phases > 1 ? (uint32_t)splits : 0u;
 }
 
 Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool backward) {
@@ -402,6 +437,13 @@ Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool b
     p.wd = take(2ull * p.np * O * p.Fp);
     p.x = take(2ull * p.np * p.chunk * p.Dp);
     p.h = take(2ull * p.np * p.chunk * p.Fp);
+    const uint32_t cols = backward ? D : O, phases = backward ? 2u : 1u;
+    if (p.chunk == M) p.product_splits = product_splits(M, cols, F, phases, p.np);
+    if (p.product_splits) {
+        p.product_per_split = (uint32_t)round_up64(ceil_div(F, p.product_splits), 64);
+        p.product_splits = ceil_div(F, p.product_per_split);
+        p.product_part = take(4ull * p.product_splits * phases * M * cols);
+    }
     if (backward) {
         p.dy = take(2ull * p.np * p.chunk * p.Op);
         p.dg = take(2ull * p.np * p.chunk * p.Fp);
@@ -501,16 +543,29 @@ template <class E, int TM, int TN, int WM, int WN, bool BKC> int launch_product_
     constexpr int NP = Terms<E>::NP;
     a.col_tiles = ceil_div(a.N, (uint32_t)TN);
     a.tiles = ceil_div(a.M, (uint32_t)TM) * a.col_tiles;
-    hipLaunchKernelGGL((k_product<E, T, NP, TM, TN, WM, WN, BKC>), dim3(grid_of(a.tiles, WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
+    hipLaunchKernelGGL((k_product<E, T, NP, TM, TN, WM, WN, BKC>), dim3(grid_of((uint64_t)a.tiles * (a.splits ? a.splits * a.phases : 1u), WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
     return check_launch("k_product");
 }
 bool whole_units(const void* p, int64_t ld, uint32_t cols, uint32_t size) {
     const uint32_t unit = 16u / size;
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % unit == 0 && cols % unit == 0;
 }
-template <class E, bool BKC> int launch_product(ProductArgs a, hipStream_t s) {
+template <class E, bool BKC> int launch_product(ProductArgs a, const Plan& p, char* ws, hipStream_t s) {
     constexpr int NP = Terms<E>::NP;
     a.aligned = whole_units(a.out, a.ld, a.N, sizeof(E));
+    if (p.product_splits) {
+        a.splits = p.product_splits;
+        a.per_split = p.product_per_split;
+        a.part = reinterpret_cast<float*>(ws + p.product_part);
+        if (int rc = launch_product_as<E, 128, 128, 2, 2, BKC>(a, s)) return rc;
+        SumArgs u{};
+        u.jobs = 1;
+        u.splits = a.splits * a.phases;
+        const uint64_t n = (uint64_t)a.M * a.N;
+        u.job[0] = {a.part, a.out, n, 0, a.N, a.ld};
+        hipLaunchKernelGGL((k_sum_splits<E>), dim3((uint32_t)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, u);
+        return check_launch("k_sum_splits");
+    }
     if (!large_product(a.M, a.N, NP)) return launch_product_as<E, 128, 128, 2, 2, BKC>(a, s);
     if constexpr (NP == 1) return launch_product_as<E, 256, 256, 2, 4, BKC>(a, s);
     else return launch_product_as<E, 256, 128, 4, 2, BKC>(a, s);
@@ -600,7 +655,7 @@ template <class E> int forward(const void* x, int64_t ldx, const Weights& w, uin
         q.b[0] = owd;
         q.K = p.Fp; q.phases = 1;
         q.out = static_cast<E*>(y) + (int64_t)m0 * ldy; q.ld = ldy; q.M = rows; q.N = O;
-        if (int rc = launch_product<E, true>(q, s)) return rc;
+        if (int rc = launch_product<E, true>(q, p, ws, s)) return rc;
     }
     return ENVIDR_OK;
 }
@@ -643,7 +698,7 @@ template <class E> int backward(const void* dy, int64_t lddy, const void* x, int
             q.b[1] = strided(owu, p.Dp);
             q.K = F; q.phases = 2;
             q.out = static_cast<E*>(dx) + (int64_t)m0 * lddx; q.ld = lddx; q.M = rows; q.N = D;
-            if (int rc = launch_product<E, false>(q, s)) return rc;
+            if (int rc = launch_product<E, false>(q, p, ws, s)) return rc;
         }
         GradArgs g{};
         auto job = [&](Operand l, Operand r, void* out, uint64_t part_at, uint32_t n_rows, uint32_t n_cols) {
@@ -669,15 +724,16 @@ template <class E> int backward(const void* dy, int64_t lddy, const void* x, int
         SumArgs u{};
         u.splits = p.splits;
         uint32_t blocks = 0;
-        auto job = [&](void* out, uint64_t part_at, uint64_t n) {
+        auto job = [&](void* out, uint64_t part_at, uint32_t n_rows, uint32_t n_cols) {
             if (!out) return;
-            u.job[u.jobs++] = {part + part_at, out, n, blocks};
+            const uint64_t n = (uint64_t)n_rows * n_cols;
+            u.job[u.jobs++] = {part + part_at, out, n, blocks, n_cols, n_cols};
             blocks += (uint32_t)((n + kBlock - 1) / kBlock);
         };
         const uint64_t fd = (uint64_t)p.splits * F * D;
-        job(dwg, 0, (uint64_t)F * D);
-        job(dwu, fd, (uint64_t)F * D);
-        job(dwd, 2 * fd, (uint64_t)O * F);
+        job(dwg, 0, F, D);
+        job(dwu, fd, F, D);
+        job(dwd, 2 * fd, O, F);
         hipLaunchKernelGGL((k_sum_splits<E>), dim3(blocks), dim3(kBlock), 0, s, u);
         return check_launch("k_sum_splits");
     }
