@@ -18,26 +18,36 @@ template <class E, int N> struct __attribute__((packed, aligned(sizeof(E)))) Pac
 template <class E, int N> __device__ __forceinline__ Pack<E, N> load_pack(const E* p) { return *reinterpret_cast<const Pack<E, N>*>(p); }
 template <class E, int N> __device__ __forceinline__ void store_pack(E* p, const Pack<E, N>& v) { *reinterpret_cast<Pack<E, N>*>(p) = v; }
 
-// sigmoid(v) and sigmoid(-v), both to full relative precision at either end (1 - sigmoid would lose it where sigmoid -> 1)
-__device__ __forceinline__ void sigmoid_pair(float v, float& s, float& s_neg) {
-    const float e = expf(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
-    s = v < 0.0f ? e * r : r;
-    s_neg = v < 0.0f ? r : e * r;
-    // (a NaN takes the second branch with e = NaN: both come out NaN)
+// sigmoid(v) and sigmoid(-v), both to full relative precision at either end (1 - sigmoid would lose it where sigmoid -> 1), from one
+// exponential e = 2^(-|v| log2 e).  FINE: the product's rounding puts an error of |v| 2^-24 on e -- nothing beside the steps of 16-bit inputs
+// and results; fp32 takes the product's low part along.
+template <bool FINE> __device__ __forceinline__ void sigmoid_pair(float v, float& s, float& s_neg) {
+    float x = fabsf(v), e;
+    if constexpr (FINE) {
+        x = x > 150.0f ? 150.0f : x;                 // (e is 0 there; an infinity would make the low part NaN)
+        const float t = x * -1.44269504f, lo = fmaf(x, -1.44269504f, -t) - x * 1.92596299e-8f;
+        e = __builtin_amdgcn_exp2f(t);
+        e = fmaf(e, lo * 0.693147181f, e);
+    } else {
+        e = __builtin_amdgcn_exp2f(x * -1.44269504f);
+    }
+    const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+    s = v < 0.0f ? er : r;
+    s_neg = v < 0.0f ? r : er;                       // (a NaN: e, and so both)
 }
 
 // act(g) and act'(g)
-template <int ACT> __device__ __forceinline__ void activation(float g, float& a, float& da) {
+template <int ACT, bool FINE> __device__ __forceinline__ void activation(float g, float& a, float& da) {
     if constexpr (ACT == ENVIDR_ACT_RELU) {
         a = g < 0.0f ? 0.0f : g;                 // (NaN stays NaN)
         da = g > 0.0f ? 1.0f : 0.0f;
     } else if constexpr (ACT == ENVIDR_ACT_SIGMOID) {
         float sn;
-        sigmoid_pair(g, a, sn);
+        sigmoid_pair<FINE>(g, a, sn);
         da = a * sn;
     } else if constexpr (ACT == ENVIDR_ACT_SILU) {
         float s, sn;
-        sigmoid_pair(g, s, sn);
+        sigmoid_pair<FINE>(g, s, sn);
         a = g * s;
         da = fmaf(a, sn, s);
     } else {
@@ -45,7 +55,7 @@ template <int ACT> __device__ __forceinline__ void activation(float g, float& a,
         const float k2 = 1.5957691216057308f, c = 0.044715f;
         const float cg = g > 16.0f ? 16.0f : (g < -16.0f ? -16.0f : g), q = cg * cg;
         float s, sn;
-        sigmoid_pair(k2 * cg * fmaf(c, q, 1.0f), s, sn);
+        sigmoid_pair<FINE>(k2 * cg * fmaf(c, q, 1.0f), s, sn);
         a = g * s;
         da = fmaf(cg * s * sn, k2 * fmaf(3.0f * c, q, 1.0f), s);
     }

@@ -13,8 +13,11 @@
 // Operands that the core cannot read as they are (fp32: three bf16 terms; widths, pitches or addresses that are no multiples of 16 bytes) are
 // laid out first by k_pack_operands.  Rows go in chunks of at most kChunkBytes of hidden-layer operands.
 //
+// Narrow layers of the 16-bit types (all weights in one CU's LDS) go forward in one kernel (gated_narrow.hip).
+//
 // Up to ENVIDR_GATED_FEW_ROWS rows the weights' bytes are all there is to move: k_few_rows streams them once through registers, sixteen
 // weight rows a workgroup, the reduction split over its waves.
+#include "gated_mlp.hip.h"
 #include "gemm_core.hip.h"
 
 namespace envidr {
@@ -100,7 +103,7 @@ template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ v
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float act, slope;
-                        activation<ACT>(acc[mi + b][2 * j][r], act, slope);
+                        activation<ACT, NP == 3>(acc[mi + b][2 * j][r], act, slope);
                         h[b][j][r] = act * acc[mi + b][2 * j + 1][r];
                     }
             Out::store(scratch, h, a.h, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
@@ -110,7 +113,7 @@ template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ v
 
 template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ void __launch_bounds__(WM* WN * 64, 2) k_glu_backward(GluArgs a) {
     using P = Product<T, NP, TM, 2 * TF, WM, WN, true, true, true>;
-    using Q = Product<T, NP, TM, TF, WM, WN, true, false, false>;
+    using Q = Product<T, NP, TM, TF, WM, WN, true, false, false, TF == 96 ? 128 : TF>;
     using Out = PlaneStore<T, NP, Q::NI * 16>;
     constexpr int kStores = P::MI / Out::kBlocks * Out::kCount * 3;
     __shared__ __attribute__((aligned(1024))) char lds_all[2 * P::kStage + WM * WN * 2048];
@@ -142,7 +145,7 @@ template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ v
                     for (int r = 0; r < 4; ++r) {
                         float act, slope;
                         const float u = acc[mi + b][2 * j + 1][r], d = dh[mi + b][j][r];
-                        activation<ACT>(acc[mi + b][2 * j][r], act, slope);
+                        activation<ACT, NP == 3>(acc[mi + b][2 * j][r], act, slope);
                         h[b][j][r] = act * u;
                         dg[b][j][r] = d * u * slope;
                         du[b][j][r] = d * act;
@@ -358,7 +361,7 @@ template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWave
     for (int r = 0; r < 4; ++r) {
         if constexpr (GLU) {
             float act, slope;
-            activation<ACT>(sum[0][r], act, slope);
+            activation<ACT, sizeof(E) == 4>(sum[0][r], act, slope);
             v[r] = act * sum[1][r];
         } else {
             v[r] = sum[0][r];
@@ -428,6 +431,10 @@ Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool b
     if (!backward && M <= ENVIDR_GATED_FEW_ROWS) {
         p.h = 0;
         p.bytes = round_up64((uint64_t)M * p.Fp * dtype_size(dtype), 256);
+        return p;
+    }
+    if (!backward && gated_is_narrow(D, F, O, dtype)) {
+        p.bytes = 16;
         return p;
     }
     uint64_t at = 0;
@@ -527,14 +534,6 @@ Operand hidden(const uint16_t* p, uint32_t Fp, uint32_t rows, uint64_t plane, bo
     return {p, plane, Fp, k_strided ? Fp : rows};
 }
 
-#define ENVIDR_FOR_ACT(act, ACT, ...)                                                                  \
-    do {                                                                                               \
-        if ((act) == ENVIDR_ACT_SILU) { constexpr int ACT = ENVIDR_ACT_SILU; __VA_ARGS__; }            \
-        else if ((act) == ENVIDR_ACT_GELU) { constexpr int ACT = ENVIDR_ACT_GELU; __VA_ARGS__; }       \
-        else if ((act) == ENVIDR_ACT_RELU) { constexpr int ACT = ENVIDR_ACT_RELU; __VA_ARGS__; }       \
-        else { constexpr int ACT = ENVIDR_ACT_SIGMOID; __VA_ARGS__; }                                  \
-    } while (0)
-
 template <class E> struct Terms { using T = E; static constexpr int NP = 1; };
 template <> struct Terms<float> { using T = __bf16; static constexpr int NP = 3; };
 
@@ -598,7 +597,7 @@ template <class E, int ACT, int TM, int TF, int WM, int WN> int launch_glu_backw
 template <class E, int ACT> int launch_glu_backward(const GluArgs& a, hipStream_t s) {
     constexpr int NP = Terms<E>::NP;
     if constexpr (NP == 1) {
-        if (tiles_of(a.M, a.F, {256, 64}) >= kEnoughTiles) return launch_glu_backward_as<E, ACT, 256, 64, 4, 2>(a, s);
+        if (tiles_of(a.M, a.F, {256, 96}) >= kEnoughTiles) return launch_glu_backward_as<E, ACT, 256, 96, 4, 2>(a, s);
         return launch_glu_backward_as<E, ACT, 128, 64, 2, 2>(a, s);
     } else {
         return launch_glu_backward_as<E, ACT, 128, 64, 4, 2>(a, s);
@@ -630,6 +629,11 @@ template <class E> int forward(const void* x, int64_t ldx, const Weights& w, uin
         FewArgs d{ws, w.wd, nullptr, y, (int64_t)p.Fp, w.ldn, 0, ldy, M, F, O};
         hipLaunchKernelGGL((k_few_rows<E, ENVIDR_ACT_SILU, false>), dim3(ceil_div(O, 16u)), dim3(kFewWaves * 64), 0, s, d);
         return check_launch("k_few_rows");
+    }
+    if constexpr (NP == 1) {
+        if (gated_is_narrow(D, F, O, dtype)) {
+            return gated_narrow_forward({x, w.wg, w.wu, w.wd, y, ldx, w.lg, w.lu, w.ldn, ldy, M, D, F, O}, dtype, act, s);
+        }
     }
     Operand owg{}, owu{}, owd{};
     for (uint32_t m0 = 0; m0 < M; m0 += p.chunk) {

@@ -150,11 +150,12 @@ template <int N> __device__ __forceinline__ void tile_barrier() { asm volatile("
 // (the waves of a workgroup pass the barrier together: without this they would all read, then all multiply).
 //   barrier t: step t + 1 has landed for everyone, and everyone has the last of step t in registers, so its stage is free for step t + S
 // Steps past the end are loads of zeros: the number in flight is the same at every wait.
-template <class T, int NP, int TM, int TN, int WM, int WN, bool AKC, bool BKC, bool PAIR> struct Product {
+// (B's tile may be loaded TL wide and used TN wide: a K-strided tile's rows have to divide a bank period.)
+template <class T, int NP, int TM, int TN, int WM, int WN, bool AKC, bool BKC, bool PAIR, int TL = TN> struct Product {
     static constexpr int KT = NP == 1 ? 64 : 32;
     static constexpr int WAVES = WM * WN, MI = TM / WM / 16, NI = TN / WN / 16;
     using LA = TileLoad<TM, KT, NP, AKC, WAVES>;
-    using LB = TileLoad<TN, KT, NP, BKC, WAVES, PAIR>;
+    using LB = TileLoad<TL, KT, NP, BKC, WAVES, PAIR>;
     static constexpr int kStage = LA::kBytes + LB::kBytes;
 
     struct Fragments {
@@ -317,26 +318,27 @@ __device__ __forceinline__ void store_to_buffer(u32x4 v, void* p, uint32_t bytes
 }
 
 // Sixteen-bit results on their way out.  A wave holds, of each row of a 16-row block, four adjacent columns in each lane group: stored like
-// that a row is written 32 bytes at a time.  Through 2 KiB of LDS of its own the wave turns 1024 / COLS rows of COLS columns into whole rows.
+// that a row is written 32 bytes at a time.  Through 2 KiB of LDS of its own the wave turns kRows rows of COLS columns into whole rows.
 template <int COLS> struct RowStore {
-    static constexpr int kRows = 1024 / COLS, kUnits = COLS / 8, kBytes = 2048;
+    static constexpr int kPitch = COLS <= 16 ? 16 : COLS <= 32 ? 32 : 64;           // of a row in LDS
+    static constexpr int kRows = 1024 / kPitch, kUnits = kPitch / 8, kBytes = 2048, kStores = 2;
+    static_assert(COLS % 16 == 0 && COLS <= 64, "whole blocks");
     typedef __attribute__((address_space(3))) s16x4 lds_half;
     // columns col .. col + 3 of row `row` of the block
     static __device__ __forceinline__ void put(uint32_t lds, uint32_t row, uint32_t col, s16x4 v) {
         const uint32_t unit = (col >> 3) ^ (row & (kUnits - 1u));
-        *(lds_half*)(lds + row * (COLS * 2u) + unit * 16u + (col & 4u) * 2u) = v;
+        *(lds_half*)(lds + row * (kPitch * 2u) + unit * 16u + (col & 4u) * 2u) = v;
     }
-    static constexpr int kStores = 2;
     // the block's rows to p (its first row, `rows` of them there) from column col0 on (`cols` of them there): 16-byte aligned, whole units.
     // Always kStores memory operations.
     static __device__ __forceinline__ void flush(uint32_t lds, uint16_t* p, uint32_t ld, uint32_t rows, uint32_t col0, uint32_t cols) {
         const uint32_t lane = threadIdx.x & 63u;
         const uint32_t bytes = min(rows, (uint32_t)kRows) * ld * 2u;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < kStores; ++j) {
             const uint32_t idx = j * 64u + lane, row = idx / kUnits, unit = idx % kUnits, col = col0 + unit * 8u;
-            const u32x4 v = *(const lds_u32x4*)(lds + row * (COLS * 2u) + (unit ^ (row & (kUnits - 1u))) * 16u);
-            store_to_buffer(v, p, bytes, col < cols ? (row * ld + col) * 2u : kOutside);
+            const u32x4 v = *(const lds_u32x4*)(lds + row * (kPitch * 2u) + (unit ^ (row & (kUnits - 1u))) * 16u);
+            store_to_buffer(v, p, bytes, unit * 8u < (uint32_t)COLS && col < cols ? (row * ld + col) * 2u : kOutside);
         }
     }
 };

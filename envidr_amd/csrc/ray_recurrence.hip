@@ -113,23 +113,6 @@ __global__ void __launch_bounds__(kBlock) k_scan_map(ScanArgs a) {
         for (uint32_t k = r.begin / a.piece + 1u + lane; k <= (r.end - 1u) / a.piece; k += 64u) a.owner[k] = (int32_t)n;
 }
 
-// sigmoid(v) and sigmoid(-v) from one exponential, e = 2^(-|v| log2 e).  The product's rounding puts an error of |v| 2^-24 on e: nothing beside
-// a 16-bit gate's own steps; fp32 gates take the product's low part along.
-template <class E> __device__ __forceinline__ void gate_pair(float v, float& s, float& s_neg) {
-    float x = fabsf(v), e;
-    if constexpr (sizeof(E) == 4) {
-        x = x > 150.0f ? 150.0f : x;                 // (e is 0 there; an infinity would make the low part NaN)
-        const float t = x * -1.44269504f, lo = fmaf(x, -1.44269504f, -t) - x * 1.92596299e-8f;
-        e = __builtin_amdgcn_exp2f(t);
-        e = fmaf(e, lo * 0.693147181f, e);
-    } else {
-        e = __builtin_amdgcn_exp2f(x * -1.44269504f);
-    }
-    const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
-    s = v < 0.0f ? er : r;
-    s_neg = v < 0.0f ? r : er;                       // (a NaN: e, and so both)
-}
-
 // UNI: a wave has one piece, so what depends on the piece is the same for all lanes
 template <bool UNI> __device__ __forceinline__ uint32_t same(uint32_t v) { return UNI ? (uint32_t)__builtin_amdgcn_readfirstlane((int)v) : v; }
 
@@ -286,7 +269,7 @@ template <class E, int V, bool BLEND, bool UNI> __global__ void __launch_bounds_
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     float s, sn;
-                    gate_pair<E>(x.g.at(j, i), s, sn);
+                    sigmoid_pair<sizeof(E) == 4>(x.g.at(j, i), s, sn);
                     h[i] = step<BLEND>(h[i], s, sn, x.v.at(j, i));
                 }
                 store_row<E, V>(a.out0, row, a.C, p.c, h);
@@ -338,7 +321,7 @@ template <class E, int V, bool BLEND, bool UNI> __global__ void __launch_bounds_
                 for (int i = 0; i < V; ++i) {
                     before[j][i] = x.h[i];
                     float s, sn;
-                    gate_pair<E>(x.g.at(j, i), s, sn);
+                    sigmoid_pair<sizeof(E) == 4>(x.g.at(j, i), s, sn);
                     const float then = step<BLEND>(x.h[i], s, sn, x.v.at(j, i));
                     x.h[i] = row >= p.begin ? then : x.h[i];
                 }
@@ -353,7 +336,7 @@ template <class E, int V, bool BLEND, bool UNI> __global__ void __launch_bounds_
                     // (formed again: kept from the pass above, the pairs would take 32 V registers more and halve the waves in flight)
                     float s, sn, gate = x.g.at(j, i);
                     asm("" : "+v"(gate));
-                    gate_pair<E>(gate, s, sn);
+                    sigmoid_pair<sizeof(E) == 4>(gate, s, sn);
                     const float G = x.d.at(j, i) + e[i], from = BLEND ? before[j][i] - x.v.at(j, i) : before[j][i];
                     dv[i] = BLEND ? G * sn : G;
                     e[i] = s * G;
@@ -405,7 +388,7 @@ template <class E, int V, bool BLEND, bool BACK, bool UNI> __global__ void __lau
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float s, sn;
-                gate_pair<E>(x.g.at(j, i), s, sn);
+                sigmoid_pair<sizeof(E) == 4>(x.g.at(j, i), s, sn);
                 const float y = x.v.at(j, i);
                 B[i] = BACK ? s * (B[i] + y) : step<BLEND>(B[i], s, sn, y);
                 A[i] *= s;
