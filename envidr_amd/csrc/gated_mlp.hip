@@ -399,6 +399,10 @@ uint64_t tiles_of(uint64_t rows, uint64_t cols, TileSize t) { return (rows + t.m
 constexpr TileSize product_tile(uint32_t np, bool large) { return large ? (np == 1 ? TileSize{256, 256} : TileSize{256, 128}) : TileSize{128, 128}; }
 bool large_product(uint64_t rows, uint64_t cols, uint32_t np) { return tiles_of(rows, cols, product_tile(np, true)) >= kEnoughTiles; }
 uint64_t grad_tiles(uint32_t D, uint32_t F, uint32_t O, TileSize t) { return 2 * tiles_of(F, D, t) + tiles_of(O, F, t); }
+// workgroups a CU holds: by the LDS of two stages of a (rows + cols)-wide tile and the waves' 2 KiB
+constexpr uint32_t per_cu(int np, int rows, int cols, int waves) {
+    return 2 * (2 * np * (rows + cols) * (np == 1 ? 64 : 32) * 2 + waves * 2048) <= 160 * 1024 ? 2u : 1u;
+}
 // workgroups: as many as are resident at once, in whole rounds of the XCDs
 uint32_t grid_of(uint64_t tiles, uint32_t per_cu) {
     const uint64_t all = (tiles + 7) / 8 * 8, most = (uint64_t)kCus * per_cu;
@@ -542,7 +546,7 @@ template <class E, int TM, int TN, int WM, int WN, bool BKC> int launch_product_
     constexpr int NP = Terms<E>::NP;
     a.col_tiles = ceil_div(a.N, (uint32_t)TN);
     a.tiles = ceil_div(a.M, (uint32_t)TM) * a.col_tiles;
-    hipLaunchKernelGGL((k_product<E, T, NP, TM, TN, WM, WN, BKC>), dim3(grid_of((uint64_t)a.tiles * (a.splits ? a.splits * a.phases : 1u), WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
+    hipLaunchKernelGGL((k_product<E, T, NP, TM, TN, WM, WN, BKC>), dim3(grid_of((uint64_t)a.tiles * (a.splits ? a.splits * a.phases : 1u), per_cu(NP, TM, TN, WM * WN))), dim3(WM * WN * 64), 0, s, a);
     return check_launch("k_product");
 }
 bool whole_units(const void* p, int64_t ld, uint32_t cols, uint32_t size) {
@@ -575,7 +579,7 @@ template <class E, int ACT, int TM, int TF, int WM, int WN> int launch_glu_forwa
     constexpr int NP = Terms<E>::NP;
     a.col_tiles = ceil_div(a.F, (uint32_t)TF);
     a.tiles = ceil_div(a.M, (uint32_t)TM) * a.col_tiles;
-    hipLaunchKernelGGL((k_glu_forward<T, NP, TM, TF, WM, WN, ACT>), dim3(grid_of(a.tiles, WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
+    hipLaunchKernelGGL((k_glu_forward<T, NP, TM, TF, WM, WN, ACT>), dim3(grid_of(a.tiles, per_cu(NP, TM, 2 * TF, WM * WN))), dim3(WM * WN * 64), 0, s, a);
     return check_launch("k_glu_forward");
 }
 template <class E, int ACT> int launch_glu_forward(const GluArgs& a, hipStream_t s) {
@@ -590,7 +594,7 @@ template <class E, int ACT, int TM, int TF, int WM, int WN> int launch_glu_backw
     constexpr int NP = Terms<E>::NP;
     a.col_tiles = ceil_div(a.F, (uint32_t)TF);
     a.tiles = ceil_div(a.M, (uint32_t)TM) * a.col_tiles;
-    hipLaunchKernelGGL((k_glu_backward<T, NP, TM, TF, WM, WN, ACT>), dim3(grid_of(a.tiles, WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
+    hipLaunchKernelGGL((k_glu_backward<T, NP, TM, TF, WM, WN, ACT>), dim3(grid_of(a.tiles, per_cu(NP, TM, 2 * TF, WM * WN))), dim3(WM * WN * 64), 0, s, a);
     return check_launch("k_glu_backward");
 }
 // (three accumulators a hidden unit: half the columns of the other products)
@@ -600,14 +604,14 @@ template <class E, int ACT> int launch_glu_backward(const GluArgs& a, hipStream_
         if (tiles_of(a.M, a.F, {256, 96}) >= kEnoughTiles) return launch_glu_backward_as<E, ACT, 256, 96, 4, 2>(a, s);
         return launch_glu_backward_as<E, ACT, 128, 64, 2, 2>(a, s);
     } else {
-        return launch_glu_backward_as<E, ACT, 128, 64, 4, 2>(a, s);
+        return launch_glu_backward_as<E, ACT, 256, 64, 4, 2>(a, s);
     }
 }
 
 template <class E, int TM, int TN, int WM, int WN> int launch_weight_grads_as(const GradArgs& a, hipStream_t s) {
     using T = typename Terms<E>::T;
     constexpr int NP = Terms<E>::NP;
-    hipLaunchKernelGGL((k_weight_grads<E, T, NP, TM, TN, WM, WN>), dim3(grid_of((uint64_t)a.tiles * a.splits, WM * WN == 4 && NP == 1 ? 2 : 1)), dim3(WM * WN * 64), 0, s, a);
+    hipLaunchKernelGGL((k_weight_grads<E, T, NP, TM, TN, WM, WN>), dim3(grid_of((uint64_t)a.tiles * a.splits, per_cu(NP, TM, TN, WM * WN))), dim3(WM * WN * 64), 0, s, a);
     return check_launch("k_weight_grads");
 }
 template <class E> int launch_weight_grads(const GradArgs& a, bool large, hipStream_t s) {

@@ -23,8 +23,13 @@ __device__ __forceinline__ uint32_t narrow_swizzle(uint32_t units, uint32_t row)
     return p ^ ((units == 4u ? p ^ (p >> 1) : units == 8u ? (p >> 1) ^ (p >> 2) : (p >> 2) ^ (p >> 3)) & 1u);
 }
 
-// eight adjacent elements from column k of a row of n; zeros behind it
-template <class E> __device__ __forceinline__ s16x8 load8(const E* row, uint32_t k, uint32_t n) {
+// Eight adjacent elements from column k of a row of n; zeros behind it.  whole: n is a multiple of 8, and a load behind it is a load of the last
+// eight instead, made zero: no branch, so that loads can go out together.
+template <class E> __device__ __forceinline__ s16x8 load8(const E* row, uint32_t k, uint32_t n, bool whole) {
+    if (whole) {
+        const s16x8 v = __builtin_bit_cast(s16x8, load_pack<E, 8>(row + min(k, n - 8u)));
+        return k < n ? v : s16x8{};
+    }
     if (k + 8u <= n) return __builtin_bit_cast(s16x8, load_pack<E, 8>(row + k));
     Pack<E, 8> v;
 #pragma unroll
@@ -40,13 +45,36 @@ template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(kN
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)lds_all, lane = threadIdx.x & 63u, g = lane >> 4, i = lane & 15u;
     const uint32_t hidden = (a.F + 31u) / 32u * 32u, down = lds + 2u * hidden * kUnits * 16u, down_units = narrow_down_units(hidden);
     const E *wg = static_cast<const E*>(a.wg), *wu = static_cast<const E*>(a.wu), *wd = static_cast<const E*>(a.wd);
-    // weights: blocks of 16 rows, per 32 hidden units gate, gate, up, up
-    for (uint32_t at = threadIdx.x; at < 2u * hidden * (KD * 4u); at += kNarrowWaves * 64) {
-        const uint32_t row = at / (KD * 4u), unit = at % (KD * 4u), f = (row >> 6) * 32u + (row & 31u);
-        const bool up = row & 32u;
-        s16x8 v = {};
-        if (f < a.F) v = load8(up ? wu + (int64_t)f * a.lu : wg + (int64_t)f * a.lg, unit * 8u, a.D);
-        *(lds_s16x8*)(lds + (row * kUnits + (unit ^ narrow_swizzle(kUnits, row))) * 16u) = v;
+    const bool whole = a.D % 8u == 0u;
+    const uint32_t tiles = (a.M + kNarrowRows - 1u) / kNarrowRows, by = gridDim.x * kNarrowWaves;
+    // (tile t is wave t / gridDim's of workgroup t % gridDim: what is left of a round is spread over all CUs)
+    uint32_t t = (threadIdx.x >> 6) * gridDim.x + blockIdx.x;
+    struct Rows {
+        s16x8 x[MI][KD];
+    } now, next;
+    auto fetch = [&](Rows& r, uint32_t t) {
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
+            const E* row = static_cast<const E*>(a.x) + (int64_t)min(t * kNarrowRows + mi * 16u + i, a.M - 1u) * a.ldx;
+#pragma unroll
+            for (int kk = 0; kk < KD; ++kk) r.x[mi][kk] = load8(row, kk * 32u + g * 8u, a.D, whole);
+        }
+    };
+    if (t < tiles) fetch(now, t);
+    // weights: blocks of 16 rows, per 32 hidden units gate, gate, up, up; a batch's loads before its stores
+    constexpr uint32_t kThreads = kNarrowWaves * 64, kBatch = 6;
+    for (uint32_t first = threadIdx.x; first < 2u * hidden * (KD * 4u); first += kBatch * kThreads) {
+        s16x8 v[kBatch];
+        uint32_t to[kBatch];
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t at = min(first + b * kThreads, 2u * hidden * (KD * 4u) - 1u), row = at / (KD * 4u), unit = at % (KD * 4u), f = (row >> 6) * 32u + (row & 31u), fc = min(f, a.F - 1u);
+            v[b] = load8(row & 32u ? wu + (int64_t)fc * a.lu : wg + (int64_t)fc * a.lg, unit * 8u, a.D, whole);
+            if (f >= a.F) v[b] = s16x8{};
+            to[b] = lds + (row * kUnits + (unit ^ narrow_swizzle(kUnits, row))) * 16u;
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) *(lds_s16x8*)to[b] = v[b];         // (past the end: the last unit again)
     }
     for (uint32_t at = threadIdx.x; at < OB * 16u * (hidden / 8u); at += kNarrowWaves * 64) {
         const uint32_t o = at / (hidden / 8u), unit = at % (hidden / 8u), f = unit / 4u * 32u + 4u * (unit % 4u);
@@ -59,18 +87,6 @@ template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(kN
         *(lds_s16x8*)(down + (o * down_units + (unit ^ narrow_swizzle(4u, o))) * 16u) = __builtin_bit_cast(s16x8, v);
     }
     __syncthreads();
-    const uint32_t tiles = (a.M + kNarrowRows - 1u) / kNarrowRows, by = gridDim.x * kNarrowWaves;
-    struct Rows {
-        s16x8 x[MI][KD];
-    } now, next;
-    auto fetch = [&](Rows& r, uint32_t t) {
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-            const E* row = static_cast<const E*>(a.x) + (int64_t)min(t * kNarrowRows + mi * 16u + i, a.M - 1u) * a.ldx;
-#pragma unroll
-            for (int kk = 0; kk < KD; ++kk) r.x[mi][kk] = load8(row, kk * 32u + g * 8u, a.D);
-        }
-    };
     auto work = [&](const Rows& r, uint32_t t) {
         f32x4 y[MI][OB] = {};
         for (uint32_t hb = 0; hb < hidden / 32u; ++hb) {
@@ -116,9 +132,7 @@ template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(kN
             }
         }
     };
-    uint32_t t = blockIdx.x * kNarrowWaves + (threadIdx.x >> 6);
     if (t >= tiles) return;
-    fetch(now, t);
     for (;;) {
         if (t + by < tiles) fetch(next, t + by);
         work(now, t);
