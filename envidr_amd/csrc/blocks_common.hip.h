@@ -61,6 +61,20 @@ template <int ACT, bool FINE> __device__ __forceinline__ void activation(float g
     }
 }
 
+// act(g) alone (forward).  For 16-bit results the one-sided sigmoid 1 / (1 + 2^(-v log2 e)) does: it overflows to 0 where it should.
+template <int ACT, bool FINE> __device__ __forceinline__ float activation_value(float g) {
+    if constexpr (FINE || ACT == ENVIDR_ACT_RELU) {
+        float a, da;
+        activation<ACT, FINE>(g, a, da);
+        return a;
+    } else {
+        float z = g;
+        if constexpr (ACT == ENVIDR_ACT_GELU) z = 1.5957691216057308f * g * fmaf(0.044715f, g * g, 1.0f);
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+        return ACT == ENVIDR_ACT_SIGMOID ? s : g * s;
+    }
+}
+
 #define ENVIDR_FOR_DTYPE(dtype, E, ...)                                  \
     do {                                                                 \
         if ((dtype) == ENVIDR_F32) { using E = float; __VA_ARGS__; }     \

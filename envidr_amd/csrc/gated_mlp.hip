@@ -102,9 +102,7 @@ template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ v
                 for (int j = 0; j < P::NI / 2; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        float act, slope;
-                        activation<ACT, NP == 3>(acc[mi + b][2 * j][r], act, slope);
-                        h[b][j][r] = act * acc[mi + b][2 * j + 1][r];
+                        h[b][j][r] = activation_value<ACT, NP == 3>(acc[mi + b][2 * j][r]) * acc[mi + b][2 * j + 1][r];
                     }
             Out::store(scratch, h, a.h, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
         }
@@ -360,9 +358,7 @@ template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWave
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         if constexpr (GLU) {
-            float act, slope;
-            activation<ACT, sizeof(E) == 4>(sum[0][r], act, slope);
-            v[r] = act * sum[1][r];
+            v[r] = activation_value<ACT, sizeof(E) == 4>(sum[0][r]) * sum[1][r];
         } else {
             v[r] = sum[0][r];
         }

@@ -14,7 +14,10 @@
 namespace envidr {
 namespace {
 
-constexpr int kNarrowWaves = 8, kNarrowLds = 160 * 1024, kNarrowRows = 32;
+constexpr int kNarrowLds = 160 * 1024, kNarrowRows = 32;
+// waves of a workgroup: sixteen where 128 registers are enough (a wave alone waits for its own chain of products and exponentials: 99991 rows of
+// 72 -> 256 -> 12 take 27 us with eight), else eight
+constexpr int narrow_waves(int kd, int ob) { return kd <= 3 && ob == 1 ? 16 : 8; }
 constexpr uint32_t narrow_units(uint32_t kd) { return kd == 1 ? 4u : kd == 2 ? 8u : 16u; }          // 16-byte units of a weight row in LDS
 __host__ __device__ inline uint32_t narrow_down_units(uint32_t hidden) { return hidden / 8u + (20u - hidden / 8u % 16u) % 16u; }      // of a row of Wd: 4 mod 16
 
@@ -38,7 +41,8 @@ template <class E> __device__ __forceinline__ s16x8 load8(const E* row, uint32_t
 }
 
 // KD: k blocks of 32 of the input width; OB: blocks of 16 of the output width
-template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(kNarrowWaves * 64, 2) k_narrow_forward(NarrowArgs a) {
+template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(narrow_waves(KD, OB) * 64, narrow_waves(KD, OB) / 4) k_narrow_forward(NarrowArgs a) {
+    constexpr int kNarrowWaves = narrow_waves(KD, OB);
     constexpr int MI = kNarrowRows / 16;
     constexpr uint32_t kUnits = narrow_units(KD);
     __shared__ __attribute__((aligned(1024))) char lds_all[kNarrowLds];
@@ -107,9 +111,7 @@ template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(kN
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        float act, slope;
-                        activation<ACT, false>(p[mi][b][q], act, slope);
-                        v.v[4 * b + q] = from_f32<E>(act * p[mi][b + 2][q]);
+                        v.v[4 * b + q] = from_f32<E>(activation_value<ACT, false>(p[mi][b][q]) * p[mi][b + 2][q]);
                     }
                 h[mi] = __builtin_bit_cast(s16x8, v);
             }
@@ -144,8 +146,8 @@ template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(kN
 }
 
 template <class E, int ACT> int launch_narrow(const NarrowArgs& a, hipStream_t s) {
-    const uint32_t tiles = ceil_div(a.M, (uint32_t)kNarrowRows), blocks = ceil_div(tiles, (uint32_t)kNarrowWaves), grid = blocks < 256u ? blocks : 256u;
-    auto go = [&](auto kd, auto ob) { hipLaunchKernelGGL((k_narrow_forward<E, ACT, decltype(kd)::value, decltype(ob)::value>), dim3(grid), dim3(kNarrowWaves * 64), 0, s, a); };
+    const uint32_t tiles = ceil_div(a.M, (uint32_t)kNarrowRows), grid = tiles < 256u ? tiles : 256u;
+    auto go = [&](auto kd, auto ob) { hipLaunchKernelGGL((k_narrow_forward<E, ACT, decltype(kd)::value, decltype(ob)::value>), dim3(grid), dim3(narrow_waves(decltype(kd)::value, decltype(ob)::value) * 64), 0, s, a); };
     auto with_kd = [&](auto kd) {
         if (a.O <= 16) go(kd, std::integral_constant<int, 1>{});
         else go(kd, std::integral_constant<int, 4>{});
