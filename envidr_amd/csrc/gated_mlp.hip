@@ -20,6 +20,8 @@
 #include "gated_mlp.hip.h"
 #include "gemm_core.hip.h"
 
+#include <type_traits>
+
 namespace envidr {
 namespace {
 
@@ -311,37 +313,51 @@ struct FewArgs {
 };
 constexpr int kFewWaves = 8;
 
-// sixteen weight rows (of one or of both matrices) x all rows of a; every wave takes every kFewWaves-th step of the reduction
+// Sixteen weight rows (of one or of both matrices) x all rows of a; every wave takes every kFewWaves-th step of the reduction.
+// GLU: a is x, the result h in 32 bits; else a is that h, for the 16-bit matrix cores as two terms of the type (rounded, and what the rounding
+// left): the weights' bytes are what counts here, and y then has its own rounding only.
 template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWaves * 64) k_few_rows(FewArgs f) {
-    constexpr int W = 16 / sizeof(E);                    // elements of a lane's 16 bytes
+    using A = typename std::conditional<GLU, E, float>::type;
+    using Out = typename std::conditional<GLU, float, E>::type;
+    constexpr int W = 16 / sizeof(E);                    // elements of a lane's 16 bytes of weights
     constexpr uint32_t kStep = 4 * W;                    // k of a wave's step: four lane groups
     constexpr int kMats = GLU ? 2 : 1;
     __shared__ f32x4 part[kMats][kFewWaves][64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15u, n0 = blockIdx.x * 16u;
-    const E* a = static_cast<const E*>(f.a) + (int64_t)min(i, f.M - 1u) * f.lda;
+    const A* a = static_cast<const A*>(f.a) + (int64_t)min(i, f.M - 1u) * f.lda;
     const uint32_t wr = min(n0 + i, f.N - 1u);
     const E* w[kMats];
     w[0] = static_cast<const E*>(f.w) + (int64_t)wr * f.ldw;
     if constexpr (GLU) w[1] = static_cast<const E*>(f.w2) + (int64_t)wr * f.ldw2;
     f32x4 acc[kMats] = {};
-    auto fetch = [&](const E* p, uint32_t k) {
-        if (k + W <= f.K) return load_pack<E, W>(p + k);
-        Pack<E, W> v;
+    auto fetch = [&](const auto* p, uint32_t k) {
+        using P = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+        if (k + W <= f.K) return load_pack<P, W>(p + k);
+        Pack<P, W> v;
 #pragma unroll
-        for (int q = 0; q < W; ++q) v.v[q] = k + q < f.K ? p[k + q] : from_f32<E>(0.0f);
+        for (int q = 0; q < W; ++q) v.v[q] = k + q < f.K ? p[k + q] : from_f32<P>(0.0f);
         return v;
     };
     for (uint32_t k0 = wave * kStep; k0 < f.K; k0 += kFewWaves * kStep) {
         const uint32_t k = k0 + g * W;
-        const Pack<E, W> x = fetch(a, k);
+        const Pack<A, W> x = fetch(a, k);
 #pragma unroll
         for (int m = 0; m < kMats; ++m) {
             const Pack<E, W> y = fetch(w[m], k);
             if constexpr (sizeof(E) == 4) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(y.v[q], x.v[q], acc[m], 0, 0, 0);
-            } else {
+            } else if constexpr (GLU) {
                 acc[m] = mfma16<E>(__builtin_bit_cast(s16x8, y), __builtin_bit_cast(s16x8, x), acc[m]);
+            } else {
+                Pack<E, W> hi, lo;
+#pragma unroll
+                for (int q = 0; q < W; ++q) {
+                    hi.v[q] = from_f32<E>(x.v[q]);
+                    lo.v[q] = from_f32<E>(x.v[q] - to_f32(hi.v[q]));
+                }
+                acc[m] = mfma16<E>(__builtin_bit_cast(s16x8, y), __builtin_bit_cast(s16x8, lo), acc[m]);
+                acc[m] = mfma16<E>(__builtin_bit_cast(s16x8, y), __builtin_bit_cast(s16x8, hi), acc[m]);
             }
         }
     }
@@ -357,14 +373,11 @@ template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWave
     float v[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        if constexpr (GLU) {
-            v[r] = activation_value<ACT, sizeof(E) == 4>(sum[0][r]) * sum[1][r];
-        } else {
-            v[r] = sum[0][r];
-        }
+        if constexpr (GLU) v[r] = activation_value<ACT, true>(sum[0][r]) * sum[1][r];
+        else v[r] = sum[0][r];
     }
     const uint32_t n = n0 + 4u * g;
-    store_row4(static_cast<E*>(f.out) + (int64_t)i * f.ldo + n, (int64_t)f.N - n, v);
+    store_row4(static_cast<Out*>(f.out) + (int64_t)i * f.ldo + n, (int64_t)f.N - n, v);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
@@ -430,7 +443,7 @@ Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool b
     if (p.chunk > M) p.chunk = M;
     if (!backward && M <= ENVIDR_GATED_FEW_ROWS) {
         p.h = 0;
-        p.bytes = round_up64((uint64_t)M * p.Fp * dtype_size(dtype), 256);
+        p.bytes = round_up64(4ull * M * p.Fp, 256);
         return p;
     }
     if (!backward && gated_is_narrow(D, F, O, dtype)) {
