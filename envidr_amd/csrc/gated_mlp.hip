@@ -15,8 +15,8 @@
 //
 // Narrow layers of the 16-bit types (all weights in one CU's LDS) go forward in one kernel (gated_narrow.hip).
 //
-// Up to ENVIDR_GATED_FEW_ROWS rows the weights' bytes are all there is to move: k_few_rows streams them once through registers, sixteen
-// weight rows a workgroup, the reduction split over its waves.
+// Of few rows the weights' bytes are all there is to move: k_few_rows streams them once through registers, sixteen weight rows a workgroup, the
+// reduction split over its waves.
 #include "gated_mlp.hip.h"
 #include "gemm_core.hip.h"
 
@@ -313,10 +313,10 @@ struct FewArgs {
 };
 constexpr int kFewWaves = 8;
 
-// Sixteen weight rows (of one or of both matrices) x all rows of a; every wave takes every kFewWaves-th step of the reduction.
+// Sixteen weight rows (of one or of both matrices) x all rows of a (MT blocks of 16); every wave takes every kFewWaves-th step of the reduction.
 // GLU: a is x, the result h in 32 bits; else a is that h, for the 16-bit matrix cores as two terms of the type (rounded, and what the rounding
 // left): the weights' bytes are what counts here, and y then has its own rounding only.
-template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWaves * 64) k_few_rows(FewArgs f) {
+template <class E, int ACT, bool GLU, int MT> __global__ void __launch_bounds__(kFewWaves * 64) k_few_rows(FewArgs f) {
     using A = typename std::conditional<GLU, E, float>::type;
     using Out = typename std::conditional<GLU, float, E>::type;
     constexpr int W = 16 / sizeof(E);                    // elements of a lane's 16 bytes of weights
@@ -324,12 +324,14 @@ template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWave
     constexpr int kMats = GLU ? 2 : 1;
     __shared__ f32x4 part[kMats][kFewWaves][64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15u, n0 = blockIdx.x * 16u;
-    const A* a = static_cast<const A*>(f.a) + (int64_t)min(i, f.M - 1u) * f.lda;
+    const A* a[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) a[t] = static_cast<const A*>(f.a) + (int64_t)min(16u * t + i, f.M - 1u) * f.lda;
     const uint32_t wr = min(n0 + i, f.N - 1u);
     const E* w[kMats];
     w[0] = static_cast<const E*>(f.w) + (int64_t)wr * f.ldw;
     if constexpr (GLU) w[1] = static_cast<const E*>(f.w2) + (int64_t)wr * f.ldw2;
-    f32x4 acc[kMats] = {};
+    f32x4 acc[kMats][MT] = {};
     auto fetch = [&](const auto* p, uint32_t k) {
         using P = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
         if (k + W <= f.K) return load_pack<P, W>(p + k);
@@ -340,50 +342,68 @@ template <class E, int ACT, bool GLU> __global__ void __launch_bounds__(kFewWave
     };
     for (uint32_t k0 = wave * kStep; k0 < f.K; k0 += kFewWaves * kStep) {
         const uint32_t k = k0 + g * W;
-        const Pack<A, W> x = fetch(a, k);
+        Pack<E, W> y[kMats];
+        Pack<A, W> x[MT];
 #pragma unroll
-        for (int m = 0; m < kMats; ++m) {
-            const Pack<E, W> y = fetch(w[m], k);
+        for (int m = 0; m < kMats; ++m) y[m] = fetch(w[m], k);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) x[t] = fetch(a[t], k);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
             if constexpr (sizeof(E) == 4) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(y.v[q], x.v[q], acc[m], 0, 0, 0);
+                for (int m = 0; m < kMats; ++m)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[m].v[q], x[t].v[q], acc[m][t], 0, 0, 0);
             } else if constexpr (GLU) {
-                acc[m] = mfma16<E>(__builtin_bit_cast(s16x8, y), __builtin_bit_cast(s16x8, x), acc[m]);
+#pragma unroll
+                for (int m = 0; m < kMats; ++m) acc[m][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[m]), __builtin_bit_cast(s16x8, x[t]), acc[m][t]);
             } else {
                 Pack<E, W> hi, lo;
 #pragma unroll
                 for (int q = 0; q < W; ++q) {
-                    hi.v[q] = from_f32<E>(x.v[q]);
-                    lo.v[q] = from_f32<E>(x.v[q] - to_f32(hi.v[q]));
+                    hi.v[q] = from_f32<E>(x[t].v[q]);
+                    lo.v[q] = from_f32<E>(x[t].v[q] - to_f32(hi.v[q]));
                 }
-                acc[m] = mfma16<E>(__builtin_bit_cast(s16x8, y), __builtin_bit_cast(s16x8, lo), acc[m]);
-                acc[m] = mfma16<E>(__builtin_bit_cast(s16x8, y), __builtin_bit_cast(s16x8, hi), acc[m]);
+                acc[0][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[0]), __builtin_bit_cast(s16x8, lo), acc[0][t]);
+                acc[0][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[0]), __builtin_bit_cast(s16x8, hi), acc[0][t]);
             }
         }
     }
-#pragma unroll
-    for (int m = 0; m < kMats; ++m) part[m][wave][lane] = acc[m];
-    __syncthreads();
-    if (wave != 0 || i >= f.M) return;
-    f32x4 sum[kMats] = {};
-#pragma unroll
-    for (int m = 0; m < kMats; ++m)
-#pragma unroll
-        for (int q = 0; q < kFewWaves; ++q) sum[m] += part[m][q][lane];
-    float v[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        if constexpr (GLU) v[r] = activation_value<ACT, true>(sum[0][r]) * sum[1][r];
-        else v[r] = sum[0][r];
-    }
     const uint32_t n = n0 + 4u * g;
-    store_row4(static_cast<Out*>(f.out) + (int64_t)i * f.ldo + n, (int64_t)f.N - n, v);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        // (block t's sums are added up by wave t)
+#pragma unroll
+        for (int m = 0; m < kMats; ++m) part[m][wave][lane] = acc[m][t];
+        __syncthreads();
+        const uint32_t row = 16u * t + i;
+        if (wave == (uint32_t)t && row < f.M) {
+            f32x4 sum[kMats] = {};
+#pragma unroll
+            for (int m = 0; m < kMats; ++m)
+#pragma unroll
+                for (int q = 0; q < kFewWaves; ++q) sum[m] += part[m][q][lane];
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (GLU) v[r] = activation_value<ACT, true>(sum[0][r]) * sum[1][r];
+                else v[r] = sum[0][r];
+            }
+            store_row4(static_cast<Out*>(f.out) + (int64_t)row * f.ldo + n, (int64_t)f.N - n, v);
+        }
+        if (t + 1 < MT) __syncthreads();
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
 constexpr uint64_t kChunkBytes = 2ull << 30;    // of hidden-layer operands at a time
 constexpr uint32_t kMaxChunk = 1u << 22;        // rows (tile numbers stay within 32 bits at any width)
 constexpr uint32_t kMaxWidth = 1u << 20;
+
+// Rows that go forward through k_few_rows.  512 -> 2048 -> 512 and 1024 -> 4096 -> 1024 in bf16: 17 and 23 us at 16 rows, 21 and 32 at 32, 31 and 50 at
+// 64, where the tiles take 22 and 31.  256 -> 1000 -> 250 in fp32: 26 us at 64 rows, the tiles (with their three terms to lay out) 37.
+uint32_t few_rows(int dtype) { return dtype == ENVIDR_F32 ? 64u : 32u; }
 
 uint32_t pad8(uint32_t v) { return (v + 7u) / 8u * 8u; }
 
@@ -399,7 +419,8 @@ struct Plan {
 
 // Tiles.  Large: 256 x 256 by eight waves, one workgroup a CU -- LDS reads take 3/4 of the products' time where 128 x 128 by four waves takes
 // all of it (32 768 x 4096 x 1024, bf16: 1060 against 780 TFLOP/s).  The three terms of fp32 fill the LDS with 256 x 128, and six products a
-// pair of reads leave the reads' share below half.  Small where the large tiles are fewer than 3/4 of the CUs.
+// pair of reads leave the reads' share below half.  Small where the large tiles are fewer than 3/4 of the CUs: bf16 training pass of 4096 rows,
+// 512 -> 2048 -> 512: 198 us so and 279 with large tiles throughout; forward of 16 384 rows, 1024 -> 1024 -> 1024: 98 us with large ones, 113 with small.
 constexpr uint32_t kCus = 256, kEnoughTiles = 192;
 struct TileSize {
     uint32_t m, n;
@@ -441,7 +462,7 @@ Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool b
     const uint64_t most = kChunkBytes / row / 256u * 256u;
     p.chunk = (uint32_t)(most < 256u ? 256u : (most < kMaxChunk ? most : kMaxChunk));
     if (p.chunk > M) p.chunk = M;
-    if (!backward && M <= ENVIDR_GATED_FEW_ROWS) {
+    if (!backward && M <= few_rows(dtype)) {
         p.h = 0;
         p.bytes = round_up64(4ull * M * p.Fp, 256);
         return p;
@@ -635,13 +656,19 @@ template <class E> int forward(const void* x, int64_t ldx, const Weights& w, uin
     using T = typename Terms<E>::T;
     constexpr int NP = Terms<E>::NP;
     const Plan p = make_plan(M, D, F, O, dtype, false);
-    if (M <= ENVIDR_GATED_FEW_ROWS) {
-        FewArgs f{x, w.wg, w.wu, ws, ldx, w.lg, w.lu, (int64_t)p.Fp, M, D, F};
-        ENVIDR_FOR_ACT(act, ACT, hipLaunchKernelGGL((k_few_rows<E, ACT, true>), dim3(ceil_div(F, 16u)), dim3(kFewWaves * 64), 0, s, f));
-        if (int rc = check_launch("k_few_rows")) return rc;
-        FewArgs d{ws, w.wd, nullptr, y, (int64_t)p.Fp, w.ldn, 0, ldy, M, F, O};
-        hipLaunchKernelGGL((k_few_rows<E, ENVIDR_ACT_SILU, false>), dim3(ceil_div(O, 16u)), dim3(kFewWaves * 64), 0, s, d);
-        return check_launch("k_few_rows");
+    if (M <= few_rows(dtype)) {
+        const FewArgs f{x, w.wg, w.wu, ws, ldx, w.lg, w.lu, (int64_t)p.Fp, M, D, F}, d{ws, w.wd, nullptr, y, (int64_t)p.Fp, w.ldn, 0, ldy, M, F, O};
+        auto go = [&](auto mt) {
+            constexpr int MT = decltype(mt)::value;
+            ENVIDR_FOR_ACT(act, ACT, hipLaunchKernelGGL((k_few_rows<E, ACT, true, MT>), dim3(ceil_div(F, 16u)), dim3(kFewWaves * 64), 0, s, f));
+            if (int rc = check_launch("k_few_rows")) return rc;
+            hipLaunchKernelGGL((k_few_rows<E, ENVIDR_ACT_SILU, false, MT>), dim3(ceil_div(O, 16u)), dim3(kFewWaves * 64), 0, s, d);
+            return check_launch("k_few_rows");
+        };
+        if (M <= 16) return go(std::integral_constant<int, 1>{});
+        if constexpr (sizeof(E) == 4)
+            if (M > 32) return go(std::integral_constant<int, 4>{});
+        return go(std::integral_constant<int, 2>{});
     }
     if constexpr (NP == 1) {
         if (gated_is_narrow(D, F, O, dtype)) {

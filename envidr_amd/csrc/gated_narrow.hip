@@ -1,11 +1,12 @@
 // The gated feed-forward block of narrow layers, forward.
-// The shading heads' shape (72 -> 256 -> 12): all weights fit one CU's LDS, and the hidden layer never leaves the registers.  A workgroup of eight
-// waves lays the weights out in LDS once; from there on each wave takes 32 rows at a time by itself, x straight into registers (the next rows'
+// The shading heads' shape (72 -> 256 -> 12): all weights fit one CU's LDS, and the hidden layer never leaves the registers.  A workgroup
+// lays the weights out in LDS once; from there on each wave takes 32 rows at a time by itself, x straight into registers (the next rows'
 // loads under the present ones' products), 32 hidden units after the other:
 //   g, u = 2 x 2 blocks of 16 units (the four share the x operands), h = act(g) u in registers, rounded to the type;
 //   a lane holds h of units 4 g' .. 4 g' + 3 of both blocks (g' = lane / 16) for its row: exactly eight k of the next product's operand, in an
 //   order of k that Wd's rows in LDS follow, so y += h Wd^T needs no exchange between lanes.
-// Bound: the activation on the vector ALU (about 14 instructions a hidden unit and row), then the products.
+// Bound: the activation on the vector ALU (two quarter-rate instructions and about eight others a hidden unit and row), then the products.
+// 524 288 rows of 72 -> 256 -> 12 in fp16: 74 us; 99 991 rows 22 us (in two kernels, h through memory: 70).
 #include "gated_mlp.hip.h"
 #include "gemm_core.hip.h"
 

@@ -37,12 +37,11 @@ int envidr_blocks_abi_version(void);
  *   multiples of 8 and the tensors 16-byte aligned.
  * Arithmetic.  16-bit types: products on the 16-bit matrix cores, accumulated in fp32; h (forward) and dg, du, h (backward) are rounded
  * to the type once, as the next product's operands.  fp32: every operand is carried as three bf16 terms (24 significant bits), the six
- * products above 2^-24 are accumulated in fp32; an infinity in an operand gives NaN.  Up to ENVIDR_GATED_FEW_ROWS rows go through the
- * fp32 matrix cores / a kernel that streams the weights once.
+ * products above 2^-24 are accumulated in fp32; an infinity in an operand gives NaN.  Up to 32 rows (fp32: 64) go forward through a
+ * kernel that streams the weights once (fp32: on the fp32 matrix cores) and keeps h in 32 bits.
  * backward: dx [M, D], dw_gate / dw_up [F, D], dw_down [O, F] (any of them may be NULL: not computed).  It needs x, dy and the weights
  * only: g and u are formed again.
  * ------------------------------------------------------------------------------------------ */
-#define ENVIDR_GATED_FEW_ROWS 16u
 uint64_t envidr_gated_mlp_workspace_bytes(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, int backward);
 int envidr_gated_mlp_forward(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up,
                              const void* w_down, int64_t ld_down, uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, int activation,

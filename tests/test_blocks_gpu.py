@@ -27,7 +27,7 @@ def _mlp_inputs(g, dt, M, D, F, O):
 # ---- gated feed-forward block ---------------------------------------------------------------------------------------------------------------
 # one row to many, around the few-row limit and the tile edges, widths of any remainder, one-wide layers, reductions that are split (over the rows;
 # over the hidden layer), narrow layers whose weights stay in LDS
-MLP_SHAPES = [(1, 1, 1, 1), (1, 512, 2048, 512), (2, 72, 256, 12), (15, 7, 33, 5), (16, 250, 1000, 250), (17, 64, 128, 64), (63, 130, 70, 9), (127, 72, 256, 12),
+MLP_SHAPES = [(1, 1, 1, 1), (1, 512, 2048, 512), (2, 72, 256, 12), (15, 7, 33, 5), (16, 250, 1000, 250), (17, 64, 128, 64), (33, 90, 300, 20), (63, 130, 70, 9), (64, 256, 520, 256), (65, 256, 520, 256), (127, 72, 256, 12),
               (128, 128, 128, 128), (129, 8, 16, 8), (300, 257, 131, 259), (1000, 39, 64, 3), (4097, 72, 264, 16), (20011, 40, 72, 24),
               (40, 456, 944, 144), (200, 90, 2001, 77),
               (700, 128, 33, 64), (1000, 20, 900, 16), (33, 100, 250, 40)]
