@@ -234,6 +234,7 @@ template <class T, int NP, int TM, int TN, int WM, int WN, bool AKC, bool BKC, b
     // in flight while those steps are waited for -- operations complete in order, so "all but the last STORES" are the loads.
     template <int STORES, int ACC, class Turn, class Issue>
     static __device__ __forceinline__ void run(uint32_t lds, uint32_t stage_bytes, uint32_t& stage, Source& src, uint32_t n, bool relaxed, f32x4 (&acc)[MI][ACC], int at, Turn turn, Issue issue_next) {
+        static_assert(STORES < 64, "the counter of operations in flight holds 63");
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
         Fragments f[2];
         auto barrier = [&](bool first) {
@@ -321,7 +322,7 @@ __device__ __forceinline__ void store_to_buffer(u32x4 v, void* p, uint32_t bytes
 // that a row is written 32 bytes at a time.  Through 2 KiB of LDS of its own the wave turns kRows rows of COLS columns into whole rows.
 template <int COLS> struct RowStore {
     static constexpr int kPitch = COLS <= 16 ? 16 : COLS <= 32 ? 32 : 64;           // of a row in LDS
-    static constexpr int kRows = 1024 / kPitch, kUnits = kPitch / 8, kBytes = 2048, kStores = 2;
+    static constexpr int kRows = 1024 / kPitch, kUnits = kPitch / 8, kStores = 2;
     static_assert(COLS % 16 == 0 && COLS <= 64, "whole blocks");
     typedef __attribute__((address_space(3))) s16x4 lds_half;
     // columns col .. col + 3 of row `row` of the block
@@ -329,6 +330,7 @@ template <int COLS> struct RowStore {
         const uint32_t unit = (col >> 3) ^ (row & (kUnits - 1u));
         *(lds_half*)(lds + row * (kPitch * 2u) + unit * 16u + (col & 4u) * 2u) = v;
     }
+    static __device__ __forceinline__ u32x4 unit_of(uint32_t lds, uint32_t row, uint32_t unit) { return *(const lds_u32x4*)(lds + row * (kPitch * 2u) + (unit ^ (row & (kUnits - 1u))) * 16u); }
     // the block's rows to p (its first row, `rows` of them there) from column col0 on (`cols` of them there): 16-byte aligned, whole units.
     // Always kStores memory operations.
     static __device__ __forceinline__ void flush(uint32_t lds, uint16_t* p, uint32_t ld, uint32_t rows, uint32_t col0, uint32_t cols) {
@@ -337,8 +339,25 @@ template <int COLS> struct RowStore {
 #pragma unroll
         for (int j = 0; j < kStores; ++j) {
             const uint32_t idx = j * 64u + lane, row = idx / kUnits, unit = idx % kUnits, col = col0 + unit * 8u;
-            const u32x4 v = *(const lds_u32x4*)(lds + row * (kPitch * 2u) + (unit ^ (row & (kUnits - 1u))) * 16u);
-            store_to_buffer(v, p, bytes, unit * 8u < (uint32_t)COLS && col < cols ? (row * ld + col) * 2u : kOutside);
+            store_to_buffer(unit_of(lds, row, unit), p, bytes, unit * 8u < (uint32_t)COLS && col < cols ? (row * ld + col) * 2u : kOutside);
+        }
+    }
+    // the same to an output of any alignment and width (148664 x 899 of bf16: 142 us; stored four columns a lane, 32 bytes of a row at a time, 257)
+    static __device__ __forceinline__ void flush_any(uint32_t lds, uint16_t* p, int64_t ld, uint32_t rows, uint32_t col0, uint32_t cols) {
+        const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+        for (int j = 0; j < kStores; ++j) {
+            const uint32_t idx = j * 64u + lane, row = idx / kUnits, unit = idx % kUnits, col = col0 + unit * 8u;
+            const Pack<uint16_t, 8> v = __builtin_bit_cast(Pack<uint16_t, 8>, unit_of(lds, row, unit));
+            if (row >= rows || unit * 8u >= (uint32_t)COLS || col >= cols) continue;
+            uint16_t* to = p + (int64_t)row * ld + col;
+            if (cols - col >= 8u) {
+                store_pack(to, v);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 7; ++r)
+                    if (col + r < cols) to[r] = v.v[r];
+            }
         }
     }
 };
@@ -371,21 +390,21 @@ template <class E, int MI, int NI> struct ResultStore {
     static constexpr int kCount = kWide ? MI * NI : MI * 16 / RowStore<NI * 16>::kRows * 2;
     static __device__ __forceinline__ void store(uint32_t scratch, const f32x4 (&acc)[MI][NI], E* out, int64_t ld, uint32_t rows, uint32_t cols, uint32_t row0, uint32_t col0, bool aligned) {
         const uint32_t lane = threadIdx.x & 63u, i = lane & 15u, g = lane >> 4;
-        if (!aligned) {
-#pragma unroll
-            for (int mi = 0; mi < MI; ++mi) {
-                const uint32_t m = row0 + mi * 16u + i;
-                if (m >= rows) continue;
-#pragma unroll
-                for (int ni = 0; ni < NI; ++ni) {
-                    const uint32_t n = col0 + ni * 16u + 4u * g;
-                    const float v[4] = {acc[mi][ni][0], acc[mi][ni][1], acc[mi][ni][2], acc[mi][ni][3]};
-                    store_row4(out + (int64_t)m * ld + n, (int64_t)cols - n, v);
-                }
-            }
-            return;
-        }
         if constexpr (kWide) {
+            if (!aligned) {
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi) {
+                    const uint32_t m = row0 + mi * 16u + i;
+                    if (m >= rows) continue;
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni) {
+                        const uint32_t n = col0 + ni * 16u + 4u * g;
+                        const float v[4] = {acc[mi][ni][0], acc[mi][ni][1], acc[mi][ni][2], acc[mi][ni][3]};
+                        store_row4(out + (int64_t)m * ld + n, (int64_t)cols - n, v);
+                    }
+                }
+                return;
+            }
 #pragma unroll
             for (int mi = 0; mi < MI; ++mi) {
                 const uint32_t m0 = row0 + mi * 16u, left = m0 < rows ? min(rows - m0, 16u) : 0u;
@@ -405,8 +424,10 @@ template <class E, int MI, int NI> struct ResultStore {
                     W::put(scratch, mi * 16u % W::kRows + i, ni * 16u + 4u * g, pack4<E>(v));
                 }
                 if ((mi + 1) * 16 % W::kRows == 0) {
-                    const uint32_t m0 = row0 + (mi + 1) * 16u - W::kRows;
-                    W::flush(scratch, reinterpret_cast<uint16_t*>(out + (int64_t)m0 * ld), (uint32_t)ld, m0 < rows ? rows - m0 : 0u, col0, cols);
+                    const uint32_t m0 = row0 + (mi + 1) * 16u - W::kRows, left = m0 < rows ? rows - m0 : 0u;
+                    uint16_t* p = reinterpret_cast<uint16_t*>(out + (int64_t)m0 * ld);
+                    if (aligned) W::flush(scratch, p, (uint32_t)ld, left, col0, cols);
+                    else W::flush_any(scratch, p, ld, left, col0, cols);
                 }
             }
         }
