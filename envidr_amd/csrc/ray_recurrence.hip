@@ -16,9 +16,9 @@
 //                  mark nor an owner claims get zeros, and ids that no ray names keep their state
 // Short rays are one piece each and pay for none of the middle; cut rays are read twice by k_scan_sums.  With at most a row a ray or few
 // rows in all nothing is cut: two launches instead of five.
-// Lanes are channels, two each in the 16-bit types where C is even (a row of 128 channels is then one 256-byte access of a wave, not two of
-// 128: 222 us a training pass of three sequences, 300 k rows, bf16; 226 with one channel a lane).  From 64 lanes a row on a wave has one piece, and rows, bounds and addresses live on the scalar unit; with fewer channels 64 / lanes
-// pieces share a wave.
+// Lanes are channels, two each in the 16-bit types where C is even (a row of 128 channels is then one 256-byte access of a wave, not two of 128:
+// 222 us a training pass of three sequences, 300 k rows, bf16; 226 with one channel a lane).  From 64 lanes a row on a wave has one piece, and rows,
+// bounds and addresses live on the scalar unit; with fewer channels 64 / lanes pieces share a wave.
 // The backward pass needs h_{t-1}.  It does not read the stored (rounded) h: the forward pass leaves the 32-bit state at every kRows-th row
 // (`saved`), and a block's states are formed again from there in registers.
 #include "blocks_common.hip.h"
@@ -230,9 +230,12 @@ template <bool BLEND> __device__ __forceinline__ float step(float h, float a, fl
     return BLEND ? fmaf(an, v - h, h) : fmaf(a, h, v);
 }
 
-// Affine maps in order: first, then second.  A map that forgets its input (A = 0: a border of nobody, or the first border of a ray, which has the
-// ray's own initial state in B) forgets a NaN or an infinity too: what is carried there may be another ray's.
-__device__ __forceinline__ float apply(float A, float B, float in) { return A == 0.0f ? B : fmaf(A, in, B); }
+// Affine maps in order: first, then second.  A map that forgets its input -- a border of nobody, or the first border of a ray, which has the ray's
+// own initial state in B -- is marked by A = -0: what is carried there may be another ray's NaN or infinity.  (A product of sigmoids that got too
+// small is +0 and forgets nothing: a NaN stays one along its own ray.)  The mark outlives a product with a later positive A.
+constexpr float kForget = -0.0f;
+__device__ __forceinline__ bool forgets(float A) { return __builtin_bit_cast(uint32_t, A) == 0x80000000u; }
+__device__ __forceinline__ float apply(float A, float B, float in) { return forgets(A) ? B : fmaf(A, in, B); }
 
 // the state that crosses border k (forward: h before its row; backward: E behind the row before it)
 template <int V> __device__ __forceinline__ void load_carry(const ScanArgs& a, uint32_t k, uint32_t c, float (&h)[V]) {
@@ -425,7 +428,7 @@ __device__ __forceinline__ void join_runs(float* s_a, float* s_b, uint32_t run, 
         __syncthreads();
         if (run >= span) {
             B = apply(A, B, s_b[threadIdx.x - span * lanes]);
-            A *= s_a[threadIdx.x - span * lanes];
+            A = forgets(A) ? A : A * s_a[threadIdx.x - span * lanes];
         }
         __syncthreads();
     }
@@ -442,7 +445,7 @@ template <bool BACK> __global__ void __launch_bounds__(kCarryThreads) k_scan_joi
     const uint32_t k = blockIdx.x * kJoin + (BACK ? kJoin - 1u - run : run);
     const bool on = run < kJoin && c < a.C && k < a.borders;
     RayRows ray;
-    float A = 0.0f, B = 0.0f;
+    float A = kForget, B = 0.0f;
     if (on && border_owner(a, k, ray) >= 0) {
         const uint64_t at = (uint64_t)k * a.C + c;
         A = a.sum_a[at];
@@ -450,7 +453,7 @@ template <bool BACK> __global__ void __launch_bounds__(kCarryThreads) k_scan_joi
         if (k == (BACK ? (ray.end - 1u) / a.piece : ray.begin / a.piece + 1u)) {
             const float* start = BACK ? a.dlast : a.state;
             B = apply(A, B, start && ray.id >= 0 ? start[(uint64_t)(uint32_t)ray.id * a.C + c] : 0.0f);
-            A = 0.0f;
+            A = kForget;
         }
     }
     join_runs(s_a, s_b, run, runs, a.lanes, A, B);
@@ -476,7 +479,7 @@ template <bool BACK> __global__ void __launch_bounds__(kCarryThreads) k_scan_car
     for (uint32_t s0 = 0; s0 < segments; s0 += runs) {
         const uint32_t s = s0 + run, g = BACK ? segments - 1u - s : s;
         const bool mine = on && s < segments;
-        float A = 0.0f, B = 0.0f;
+        float A = kForget, B = 0.0f;
         if (mine) {
             A = a.segment_a[(uint64_t)g * a.C + c];
             B = a.segment_b[(uint64_t)g * a.C + c];

@@ -59,7 +59,7 @@ int envidr_gated_mlp_backward(const void* dy, int64_t lddy, const void* x, int64
  *   row.  A ray with count <= 0, offset < 0 or offset + count > T has no rows (the compositors' rule).
  *   state fp32 [N, C] or NULL (zeros): h before the first sample, indexed by id; last fp32 [N, C]: h after the last one.  The id of a ray
  *   without rows, and an id that no ray names, keep their state; a ray with an id outside 0 .. N-1 starts from zeros and leaves none.
- *   Rows that belong to no ray: h, dgate and dvalue are zero there.
+ *   Rows that belong to no ray: h, dgate and dvalue are zero there.  A NaN or an infinity stays with its ray and channel, and along them.
  *   saved: fp32 [envidr_ray_recurrence_saved_floats(T, N, C)] or NULL; written by the forward pass and read by the backward one of the
  *   same inputs.
  * backward: dh [T, C], dlast fp32 [N, C] or NULL -> dgate, dvalue [T, C], dstate fp32 [N, C] or NULL.

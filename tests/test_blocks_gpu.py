@@ -233,6 +233,37 @@ def test_ray_recurrence_with_saturated_gates_and_with_bad_values_elsewhere():
         assert torch.equal(h.float().cpu(), want) and torch.equal(last.cpu(), torch.tensor([[3.0], [2.5], [9.0]]).expand(3, C))
 
 
+@pytest.mark.parametrize("blend", [True, False], ids=["blend", "sum"])
+def test_ray_recurrence_keeps_a_bad_value_along_its_own_ray_only(blend):
+    """NaN and infinities in values, gates, states and gradients of long rays: from there on (backward: up to there) nothing of that ray and channel
+    is finite, however small the gates' products get, and the rays before and behind it keep their bits"""
+    from envidr_amd.blocks import ray_recurrence
+    nan, inf, T, C = float("nan"), float("inf"), 3000, 4
+    g = _gen("bad values")
+    rays = torch.tensor([[2, 2000, 990], [0, 5, 900], [1, 910, 1080]], dtype=torch.int32, device="cuda")      # (910 .. 1989: the middle one)
+    for shift in (0.0, -6.0):                                   # sigmoid(-6)^64 is below the smallest number
+        gate, value, dh = (_rand(g, torch.float32, T, C) + (shift if i == 0 else 0.0) for i in range(3))
+        state, dlast = _rand(g, torch.float32, 3, C), _rand(g, torch.float32, 3, C)
+
+        def run():
+            leaves = [t.clone().requires_grad_(True) for t in (gate, value, state)]
+            out = ray_recurrence(leaves[0], leaves[1], rays, state=leaves[2], blend=blend)
+            return [t.detach() for t in (*out, *torch.autograd.grad(out, leaves, (dh, dlast)))]
+
+        good = run()
+        value[1000, 0], gate[1100, 1], state[1, 2], dh[1800, 3] = nan, nan, inf, nan
+        bad = run()
+        others = [i for i in range(T) if not 910 <= i < 1990]
+        for a, b in zip(good, bad):
+            assert torch.equal(a[others] if len(a) == T else a[[0, 2]], b[others] if len(b) == T else b[[0, 2]])
+        h, last, _, dvalue, dstate = bad
+        for c, first in ((0, 1000), (1, 1100), (2, 910)):
+            assert not h[first:1990, c].isfinite().any() and not last[1, c].isfinite() and h[910:first, c].isfinite().all()
+        assert torch.equal(h[:, 3], good[0][:, 3])
+        for c, behind in ((1, 1101), (3, 1801)):                # channel 1: the gradient passes the NaN gate at row 1100
+            assert not dvalue[910:behind - 1, c].isfinite().any() and not dstate[1, c].isfinite() and torch.equal(dvalue[behind:, c], good[3][behind:, c])
+
+
 def test_ray_recurrence_of_nothing_and_of_rays_that_do_not_fit():
     from envidr_amd.blocks import ray_recurrence
     z = torch.zeros(0, 4, device="cuda")
