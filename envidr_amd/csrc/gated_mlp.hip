@@ -363,7 +363,8 @@ template <class E, int ACT, bool GLU, int MT> __global__ void __launch_bounds__(
 #pragma unroll
                 for (int q = 0; q < W; ++q) {
                     hi.v[q] = from_f32<E>(x[t].v[q]);
-                    lo.v[q] = from_f32<E>(x[t].v[q] - to_f32(hi.v[q]));
+                    const float rounded = to_f32(hi.v[q]);
+                    lo.v[q] = from_f32<E>(__builtin_isinf(rounded) ? 0.0f : x[t].v[q] - rounded);       // (inf - inf would be NaN)
                 }
                 acc[0][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[0]), __builtin_bit_cast(s16x8, lo), acc[0][t]);
                 acc[0][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[0]), __builtin_bit_cast(s16x8, hi), acc[0][t]);

@@ -38,7 +38,7 @@ int envidr_blocks_abi_version(void);
  * Arithmetic.  16-bit types: products on the 16-bit matrix cores, accumulated in fp32; h (forward) and dg, du, h (backward) are rounded
  * to the type once, as the next product's operands.  fp32: every operand is carried as three bf16 terms (24 significant bits), the six
  * products above 2^-24 are accumulated in fp32; an infinity in an operand gives NaN.  Up to 32 rows (fp32: 64) go forward through a
- * kernel that streams the weights once (fp32: on the fp32 matrix cores) and keeps h in 32 bits.
+ * kernel that streams the weights once (fp32: on the fp32 matrix cores) and keeps h in 32 bits.  fp16: a hidden unit above 65504 is an infinity.
  * backward: dx [M, D], dw_gate / dw_up [F, D], dw_down [O, F] (any of them may be NULL: not computed).  It needs x, dy and the weights
  * only: g and u are formed again.
  * ------------------------------------------------------------------------------------------ */
