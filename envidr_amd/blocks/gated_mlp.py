@@ -14,7 +14,9 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}      # gelu: the t
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """a matrix whose rows the kernels can walk: adjacent elements, any row pitch that keeps rows apart"""
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) <= 1 << 21 else t.contiguous()
+    if t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= 1 << 21:
+        return t
+    return t.reshape(-1).view(t.shape)          # (contiguous() would leave a matrix of one row its pitch, whatever that is)
 
 
 def _sizes(x, wg, wd):

@@ -136,6 +136,20 @@ def test_gated_mlp_hidden_units_above_the_types_largest_number():
             assert (y == sign * float("inf")).all()
 
 
+def test_gated_mlp_single_rows_with_any_pitch():
+    """a dimension of one has a stride that nothing steps by: zero, or as large as its tensor's"""
+    from envidr_amd.blocks import gated_mlp
+    g = _gen("one row")
+    big = _rand(g, torch.bfloat16, 2, (1 << 21) + 64)
+    wg, wu, wd = _rand(g, torch.bfloat16, 24, 40), _rand(g, torch.bfloat16, 24, 40), _rand(g, torch.bfloat16, 8, 24)
+    for x in (big[1:, 16:56], big[1:, 16:56].as_strided((1, 40), (0, 1)), big[:1, :40].as_strided((1, 40), (7, 1))):
+        within(gated_mlp(x, wg, wu, wd), *mlp64(x, wg, wu, wd, "silu")["y"], "y")
+    x = _rand(g, torch.bfloat16, 50, 40)
+    wg, wu = (big[i:i + 1, :40] for i in (0, 1))
+    wd = _rand(g, torch.bfloat16, 1, 9).t()
+    within(gated_mlp(x, wg, wu, wd), *mlp64(x, wg, wu, wd, "silu")["y"], "one hidden unit")
+
+
 def test_gated_mlp_in_chunks_of_rows_adds_the_weights_gradients_up():
     """more rows than one chunk of hidden-layer operands holds (2 GiB: 71 k rows of three operands of 5000 units)"""
     from envidr_amd.blocks import gated_mlp
