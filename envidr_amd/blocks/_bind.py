@@ -58,6 +58,13 @@ def same_kind(name: str, first: torch.Tensor, **others: torch.Tensor | None) -> 
     return DTYPES[first.dtype]
 
 
+def sizes(name: str, **n: int) -> None:
+    """raises unless the sizes pass through a C uint32"""
+    for what, value in n.items():
+        if value >> 32:
+            raise _lib.EnvidrError(f"{name}: {what}={value} is too large")
+
+
 class on_device:
     """The tensor's device as the current one for the launches inside (a no-op when it is already), and its current stream."""
 

@@ -25,6 +25,7 @@ def _sizes(x, wg, wd):
 
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(M, D, F, O, code, backward):
+    _bind.sizes("gated_mlp", M=M, D=D, F=F, O=O)
     return max(_bind.lib().envidr_gated_mlp_workspace_bytes(M, D, F, O, code, backward), 16)
 
 

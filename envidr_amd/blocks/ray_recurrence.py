@@ -12,6 +12,7 @@ from . import _bind
 @functools.lru_cache(maxsize=256)
 def _sizes(T, N, C):
     """bytes of the workspace, floats of what the forward pass leaves for the backward one"""
+    _bind.sizes("ray_recurrence", N=N, C=C)
     lib = _bind.lib()
     return max(lib.envidr_ray_recurrence_workspace_bytes(T, N, C), 16), lib.envidr_ray_recurrence_saved_floats(T, N, C)
 
@@ -69,7 +70,8 @@ def ray_recurrence(gate: torch.Tensor, value: torch.Tensor, rays: torch.Tensor, 
     """h_t = a_t h_{t-1} + (1 - a_t) value_t, a_t = sigmoid(gate_t), along the samples of each ray -> (h [T, C], last [N, C]).
 
     gate, value [T, C] (float32, bfloat16 or float16), rays int32 [N, 3] = (id, offset, count) as `march_rays_train` returns them: rows offset ..
-    offset + count - 1 are one ray's samples in order; rays may come in any order but share no rows.  state float32 [N, C]: h before the
+    offset + count - 1 are one ray's samples in order; rays may come in any order but share no rows and
+    no ids.  state float32 [N, C]: h before the
     first sample, by id (zeros when not given); last float32 [N, C]: h after the last one, to go on from.  blend=False: h_t = a_t h_{t-1} + value_t.
     Rows that belong to no ray, and their gradients, are zero.  States are carried in 32 bits.  Differentiable once w.r.t. gate, value and state."""
     code = _bind.same_kind("ray_recurrence", gate, value=value)
@@ -88,7 +90,8 @@ def ray_recurrence(gate: torch.Tensor, value: torch.Tensor, rays: torch.Tensor, 
 
 
 def rays_of_lengths(lengths: torch.Tensor) -> torch.Tensor:
-    """`rays` int32 [N, 3] of N sequences packed one behind the other, from their lengths [N]"""
+    """`rays` int32 [N, 3] of N sequences packed one behind the other, from their lengths [N] (none negative, below 2^31 rows in all:
+    not checked, the lengths stay on their device)"""
     count = lengths.reshape(-1).to(torch.int64)
     first = torch.cumsum(count, 0) - count
     return torch.stack([torch.arange(count.shape[0], device=count.device), first, count], 1).to(torch.int32)

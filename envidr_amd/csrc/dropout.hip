@@ -84,8 +84,9 @@ int envidr_dropout(const void* x, const void* residual, const int64_t* rng, uint
     ENVIDR_REQUIRE(p >= 0.0 && p <= 1.0, "dropout: p=%g is not a probability", p);
     if (n == 0) return ENVIDR_OK;
     ENVIDR_REQUIRE(x && rng && y, "dropout: null pointer");
+    // (a launch holds fewer than 2^32 threads)
+    ENVIDR_REQUIRE(n <= (1ull << 35) - 8ull * kBlock, "dropout: %llu elements are too many for one call", (unsigned long long)n);
     const uint64_t blocks = (n + 8ull * kBlock - 1) / (8ull * kBlock);
-    ENVIDR_REQUIRE(blocks <= 0x7FFFFFFFull, "dropout: %llu elements are too many for one call", (unsigned long long)n);
     const uint32_t limit = (uint32_t)__builtin_rint(p * 65536.0);
     const float scale = limit >= 65536u ? 0.0f : (float)(65536.0 / (65536.0 - (double)limit));
     hipStream_t s = as_stream(stream);

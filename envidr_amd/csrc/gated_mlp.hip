@@ -785,9 +785,9 @@ template <class E> int backward(const void* dy, int64_t lddy, const void* x, int
     return ENVIDR_OK;
 }
 
-__global__ void __launch_bounds__(kBlock) k_zero_bytes(uint16_t* p, uint64_t n) {
-    const uint64_t i = (uint64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (i < n) p[i] = 0;
+// n zeros; a launch holds fewer than 2^32 threads, so each walks
+__global__ void __launch_bounds__(kBlock) k_zero(uint16_t* p, uint64_t n) {
+    for (uint64_t i = (uint64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (uint64_t)gridDim.x * kBlock) p[i] = 0;
 }
 
 int gated_checks(const char* what, uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, int activation) {
@@ -842,8 +842,9 @@ int envidr_gated_mlp_backward(const void* dy, int64_t lddy, const void* x, int64
         for (int i = 0; i < 3; ++i) {
             if (!out[i]) continue;
             const uint64_t n = (uint64_t)F * (i < 2 ? D : O) * (dtype_size(dtype) / 2u);
-            hipLaunchKernelGGL(k_zero_bytes, dim3((uint32_t)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, static_cast<uint16_t*>(out[i]), n);
-            if (int rc = check_launch("k_zero_bytes")) return rc;
+            const uint64_t blocks = (n + kBlock - 1) / kBlock, most = 16 * kCus;
+            hipLaunchKernelGGL(k_zero, dim3((uint32_t)(blocks < most ? blocks : most)), dim3(kBlock), 0, s, static_cast<uint16_t*>(out[i]), n);
+            if (int rc = check_launch("k_zero")) return rc;
         }
         return ENVIDR_OK;
     }

@@ -555,7 +555,10 @@ template <class E, bool BACK> int run_scan(ScanArgs a, bool blend, void* workspa
 int scan_checks(const char* what, uint64_t T, uint32_t N, uint32_t C, int dtype, const void* workspace, uint64_t workspace_bytes) {
     ENVIDR_REQUIRE(dtype_ok(dtype), "%s: unknown dtype %d", what, dtype);
     ENVIDR_REQUIRE(C >= 1, "%s: no channels", what);
-    ENVIDR_REQUIRE(T <= 0x7FFFFFFFull && N <= 0x7FFFFFFFu && C <= (1u << 20), "%s: T=%llu, N=%u or C=%u is too large", what, (unsigned long long)T, N, C);
+    // a launch holds fewer than 2^32 threads: k_scan_map takes 64 a ray; the passes at most 64 a piece (a head of every ray, 8192 border pieces),
+    // one a row and one an id
+    const uint64_t threads = 64ull * (N + 8192ull + 8u) + T + N;
+    ENVIDR_REQUIRE(T <= 0x7FFFFFFFull && threads < 1ull << 32 && C <= (1u << 19), "%s: T=%llu, N=%u or C=%u is too large", what, (unsigned long long)T, N, C);
     ENVIDR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= envidr_ray_recurrence_workspace_bytes(T, N, C) && (workspace || (T == 0 && N == 0)),
                    "%s: workspace of %llu bytes, %llu needed", what, (unsigned long long)workspace_bytes, (unsigned long long)envidr_ray_recurrence_workspace_bytes(T, N, C));
     return ENVIDR_OK;

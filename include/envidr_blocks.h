@@ -12,7 +12,8 @@
  *     states are computed in 32 bits or more and rounded once where they are stored;
  *   - a row pitch (`ld*`) counts elements, the elements of a row are adjacent; the row pitch of an output is not below its width;
  *   - `workspace` is caller-allocated device memory, 16-byte aligned, at least the *_workspace_bytes() of the same sizes; it holds nothing
- *     between calls.  Two calls that may run at the same time (two streams, two captured graphs) need a workspace each.
+ *     between calls.  Two calls that may run at the same time (two streams, two captured graphs) need a workspace each;
+ *   - an output overlaps no input and no other output, except where it is said to.
  * Every operator may be captured into a graph (kernel launches only) and gives the same bits on every call.
  */
 #ifndef ENVIDR_BLOCKS_H
@@ -39,6 +40,7 @@ int envidr_blocks_abi_version(void);
  * to the type once, as the next product's operands.  fp32: every operand is carried as three bf16 terms (24 significant bits), the six
  * products above 2^-24 are accumulated in fp32; an infinity in an operand gives NaN.  Up to 32 rows (fp32: 64) go forward through a
  * kernel that streams the weights once (fp32: on the fp32 matrix cores) and keeps h in 32 bits.  fp16: a hidden unit above 65504 is an infinity.
+ * Limits: D, F, O <= 2^20, F D and O F <= 2^32, M < 2^31 - 256, row pitches <= 2^21.
  * backward: dx [M, D], dw_gate / dw_up [F, D], dw_down [O, F] (any of them may be NULL: not computed).  It needs x, dy and the weights
  * only: g and u are formed again.
  * ------------------------------------------------------------------------------------------ */
@@ -56,10 +58,11 @@ int envidr_gated_mlp_backward(const void* dy, int64_t lddy, const void* x, int64
  *   a_t = sigmoid(gate_t);  h_t = a_t h_{t-1} + (1 - a_t) v_t   (blend != 0)   or   a_t h_{t-1} + v_t   (blend == 0)
  *   gate, value, h [T, C]; rays int32 [N, 3] = (id, offset, count) as envidr_march_rays_train writes them: rows offset .. offset + count - 1
  *   are the samples of ray `id`, front to back.  Rays may come in any order and leave rows between and behind them; no two may share a
- *   row.  A ray with count <= 0, offset < 0 or offset + count > T has no rows (the compositors' rule).
+ *   row or an id.  A ray with count <= 0, offset < 0 or offset + count > T has no rows (the compositors' rule).
  *   state fp32 [N, C] or NULL (zeros): h before the first sample, indexed by id; last fp32 [N, C]: h after the last one.  The id of a ray
  *   without rows, and an id that no ray names, keep their state; a ray with an id outside 0 .. N-1 starts from zeros and leaves none.
  *   Rows that belong to no ray: h, dgate and dvalue are zero there.  A NaN or an infinity stays with its ray and channel, and along them.
+ *   Limits: T < 2^31, 65 N + T < 2^32 - 2^20, C <= 2^19.
  *   saved: fp32 [envidr_ray_recurrence_saved_floats(T, N, C)] or NULL; written by the forward pass and read by the backward one of the
  *   same inputs.
  * backward: dh [T, C], dlast fp32 [N, C] or NULL -> dgate, dvalue [T, C], dstate fp32 [N, C] or NULL.
@@ -79,7 +82,7 @@ int envidr_ray_recurrence_backward(const void* dh, const float* dlast, const voi
  *   y_i = residual_i + (keep_i ? x_i / (1 - q) : 0),   q = round(65536 p) / 65536,   keep_i = bits_i >= 65536 q
  *   bits_i: 16 of the 128 bits of Philox4x32-10 (Salmon et al. 2011) with key rng[0] and counter (i / 8, rng[1]), i the element's index;
  *   rng int64 [2] on the device, so a captured graph draws from whatever stands there when it is replayed.  p in [0, 1]; residual may be
- *   NULL.  The gradient is the same call on dy without a residual.  x, residual, y: n adjacent elements; y may be x or the residual.
+ *   NULL.  The gradient is the same call on dy without a residual.  x, residual, y: n <= 2^35 - 2048 adjacent elements; y may be x or the residual.
  * envidr_dropout_step: used[0..1] = rng[0..1], then rng[1] += 1 -- a call's own copy of the generator, for its backward pass.
  * ------------------------------------------------------------------------------------------ */
 int envidr_dropout(const void* x, const void* residual, const int64_t* rng, uint64_t n, double p, int dtype, void* y, envidr_stream_t stream);

@@ -1,6 +1,7 @@
 """The block operators' boundary without a GPU: the library exports what include/envidr_blocks.h declares, the binding's table is the header's,
 impossible arguments are refused before anything is launched, and the 64-bit definitions the GPU tests compare with agree with torch."""
 import ctypes
+import importlib
 import re
 from pathlib import Path
 
@@ -85,6 +86,10 @@ def test_ray_recurrence_refuses_what_it_cannot_take():
     _refused(forward(dtype=9), b"unknown dtype")
     _refused(forward(C=0), b"no channels")
     _refused(forward(T=1 << 31), b"too large")
+    _refused(forward(C=(1 << 19) + 1), b"too large")
+    _refused(forward(N=1 << 26), b"too large")                                    # 64 threads a ray: more than a launch holds
+    _refused(forward(T=(1 << 31) - 1, N=33 << 20), b"too large")
+    _refused(forward(T=(1 << 31) - 1, N=31 << 20), b"workspace")
     _refused(forward(gate=None), b"null pointer")
     _refused(forward(rays=None), b"null pointer")
     _refused(forward(last=None), b"null pointer")
@@ -110,6 +115,8 @@ def test_dropout_refuses_what_it_cannot_take():
     _refused(lib.envidr_dropout(p, None, p, 8, 1.5, 0, p, None), b"probability")
     _refused(lib.envidr_dropout(p, None, p, 8, float("nan"), 0, p, None), b"probability")
     _refused(lib.envidr_dropout(p, None, p, 8, 0.5, 7, p, None), b"unknown dtype")
+    for n in (1 << 35, (1 << 64) - 1):
+        _refused(lib.envidr_dropout(p, None, p, n, 0.5, 1, p, None), b"too many")
     _refused(lib.envidr_dropout(None, None, p, 8, 0.5, 0, p, None), b"null pointer")
     _refused(lib.envidr_dropout(p, None, None, 8, 0.5, 0, p, None), b"null pointer")
     _refused(lib.envidr_dropout_step(None, p, None), b"null pointer")
@@ -125,6 +132,11 @@ def test_the_wrappers_refuse_cpu_tensors_and_wrong_shapes():
         blocks.ray_recurrence(x, x, torch.zeros(1, 3, dtype=torch.int32))
     with pytest.raises(EnvidrError, match="GPU"):
         blocks.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64))
+    gated_mlp, ray_recurrence = (importlib.import_module(f"envidr_amd.blocks.{n}") for n in ("gated_mlp", "ray_recurrence"))
+    with pytest.raises(EnvidrError, match="M=4294967297 is too large"):
+        gated_mlp._workspace_bytes((1 << 32) + 1, 8, 8, 8, 1, 0)
+    with pytest.raises(EnvidrError, match="N=4294967296 is too large"):
+        ray_recurrence._sizes(5, 1 << 32, 4)
     with pytest.raises(EnvidrError, match="residual"):
         blocks.GatedMLP(8, 16, 4, residual=True)
     with pytest.raises(EnvidrError, match="activation"):
