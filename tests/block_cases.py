@@ -116,11 +116,11 @@ def scan64(gate, value, rays, state, blend, dt, dh=None, dlast=None):
     return out
 
 
-def philox_bits(key, call, n):
-    """16 bits an element of the Philox4x32-10 stream (Salmon et al. 2011), in unsigned 64-bit words"""
+def philox_bits(key, call, n, first=0):
+    """16 bits an element of the Philox4x32-10 stream (Salmon et al. 2011), from element `first` (a multiple of 8) on, in unsigned 64-bit words"""
     u = np.uint64
     low, half = u(0xFFFFFFFF), u(32)
-    i = np.arange((n + 7) // 8, dtype=u)
+    i = np.arange((n + 7) // 8, dtype=u) + u(first // 8)
     key, call = int(key) % 2 ** 64, int(call) % 2 ** 64
     c = [i & low, i >> half, np.full_like(i, call & 0xFFFFFFFF), np.full_like(i, call >> 32)]
     k0, k1 = key & 0xFFFFFFFF, key >> 32

@@ -511,6 +511,57 @@ def test_gated_mlp_module_trains_with_dropout_and_a_residual():
     assert torch.equal(m(x), x + gated_mlp(x, m.w_gate, m.w_up, m.w_down))
 
 
+def test_elements_beyond_32_bit_offsets():
+    """tensors of more than 2^32 elements, empty but for their ends: the ends are computed as they are alone"""
+    from envidr_amd.blocks import dropout, gated_mlp, ray_recurrence
+    dt, g = torch.bfloat16, _gen("far")
+    rows, D, F, O = (1 << 22) + 300, 1032, 64, 8
+    assert rows * D > 1 << 32
+    x, wg, wu, wd, dy = _mlp_inputs(g, dt, 300, D, F, O)
+    far, fdy = torch.zeros(rows, D, dtype=dt, device="cuda"), torch.zeros(rows, O, dtype=dt, device="cuda")
+    far[-300:], fdy[-300:] = x, dy
+    want = mlp64(x, wg, wu, wd, "silu", dy)
+    leaves = [t.requires_grad_(True) for t in (far, wg, wu, wd)]
+    y = gated_mlp(*leaves)
+    got = dict(zip(("dx", "dw_gate", "dw_up", "dw_down"), torch.autograd.grad(y, leaves, fdy)))
+    within(y[-300:], *want["y"], "y")
+    within(got["dx"][-300:], *want["dx"], "dx")
+    assert not y[:-300].any() and not got["dx"][:-300].any()
+    for name in ("dw_gate", "dw_up", "dw_down"):                # (a row of zeros adds nothing, but a sum of more terms: + rows * U of what is there)
+        value, bound = want[name]
+        within(got[name], value, bound * (1 + rows * U), name)
+    w = [t.detach() for t in (wg[:, :72].contiguous(), wu[:, :72].contiguous(), wd)]
+    with torch.no_grad():                                       # a narrow layer of rows far apart
+        y = gated_mlp(far[:, :72], *w)
+        within(y[-300:], *mlp64(x[:, :72], *w, "silu")["y"], "narrow")
+    assert not y[:-300].any()
+    del far, leaves, got, y
+
+    T, C, n = (1 << 20) + 500, 4104, 400
+    assert T * C > 1 << 32
+    gate, value = (torch.zeros(T, C, dtype=dt, device="cuda") for _ in range(2))
+    gate[-n:], value[-n:] = _rand(g, dt, n, C), _rand(g, dt, n, C)
+    rays = torch.tensor([[0, T - n, n]], dtype=torch.int32, device="cuda")
+    alone = torch.tensor([[0, 0, n]], dtype=torch.int32, device="cuda")
+    ends = [t[-n:].clone().requires_grad_(True) for t in (gate, value)]
+    leaves = [t.requires_grad_(True) for t in (gate, value)]
+    (h, last), (h1, last1) = ray_recurrence(*leaves, rays), ray_recurrence(*ends, alone)
+    dlast = torch.ones_like(last)
+    # (cut at other rows, so not the same bits: 64 steps' roundings at most of states below |value|)
+    top = float(value.abs().max())
+    assert not h[:-n].any() and float((h[-n:].float() - h1.float()).abs().max()) <= (2 ** -7 + 64 * 16 * U) * top and float((last - last1).abs().max()) <= 64 * 16 * U * top
+    one, two = torch.autograd.grad(last, leaves, dlast), torch.autograd.grad(last1, ends, dlast)
+    for a, b in zip(one, two):
+        assert not a[:-n].any() and float((a[-n:].float() - b.float()).abs().max()) <= (2 ** -7 + 64 * 16 * U) * 2 * top
+    del gate, value, leaves, h, one, a
+
+    n, key = (1 << 32) + 4099, 77
+    x = torch.ones(n, dtype=dt, device="cuda")
+    y = dropout(x, 0.5, torch.tensor([key, 3], device="cuda"))
+    first = (1 << 32) - 4096
+    assert np.array_equal(y[first:].float().cpu().numpy(), np.where(philox_bits(key, 3, n - first, first) >= 32768, 2.0, 0.0))
+
+
 def test_the_wrappers_refuse_what_does_not_fit_together():
     from envidr_amd import blocks
     from envidr_amd._lib import EnvidrError
