@@ -50,12 +50,13 @@ def same_kind(name: str, first: torch.Tensor, **others: torch.Tensor | None) -> 
     """the dtype code of `first`; raises unless it is a GPU tensor of a supported dtype and the others share its dtype and device"""
     if not first.is_cuda:
         raise _lib.EnvidrError(f"{name}: needs GPU tensors (got a {first.device} tensor); envidr_amd has no CPU path")
-    if first.dtype not in DTYPES:
-        raise _lib.EnvidrError(f"{name}: {first.dtype} is not one of {', '.join(str(d) for d in DTYPES)}")
+    dtype, device = first.dtype, first.device
+    if dtype not in DTYPES:
+        raise _lib.EnvidrError(f"{name}: {dtype} is not one of {', '.join(str(d) for d in DTYPES)}")
     for what, t in others.items():
-        if t is not None and (t.dtype != first.dtype or t.device != first.device):
-            raise _lib.EnvidrError(f"{name}: {what} is {t.dtype} on {t.device}, the first tensor {first.dtype} on {first.device}")
-    return DTYPES[first.dtype]
+        if t is not None and (t.dtype != dtype or t.device != device):
+            raise _lib.EnvidrError(f"{name}: {what} is {t.dtype} on {t.device}, the first tensor {dtype} on {device}")
+    return DTYPES[dtype]
 
 
 def sizes(name: str, **n: int) -> None:
@@ -74,10 +75,11 @@ class on_device:
         self.index = t.get_device()
 
     def __enter__(self) -> int:
-        self.before = torch.cuda.current_device()
+        # (the current device and stream as numbers: a torch.cuda.current_stream() is an object that takes as long as a small launch)
+        self.before = torch._C._cuda_getDevice()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)          # (what torch.cuda.current_stream().cuda_stream is, without the object)
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc) -> None:
         if self.before != self.index:

@@ -9,7 +9,7 @@ from . import _bind
 
 
 def _launch(x, residual, rng, p, code):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     lib = _bind.lib()
     with _bind.on_device(x) as stream:
         _bind.check(lib.envidr_dropout(x.data_ptr(), None if residual is None else residual.data_ptr(), rng.data_ptr(), x.numel(), p, code,

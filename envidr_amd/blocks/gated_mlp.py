@@ -14,7 +14,8 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}      # gelu: the t
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """a matrix whose rows the kernels can walk: adjacent elements, any row pitch that keeps rows apart"""
-    if t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= 1 << 21:
+    pitch, step = t.stride()
+    if step == 1 and t.shape[1] <= pitch <= 1 << 21:
         return t
     return t.reshape(-1).view(t.shape)          # (contiguous() would leave a matrix of one row its pitch, whatever that is)
 
@@ -33,9 +34,9 @@ def _forward(x, wg, wu, wd, code, act):
     lib = _bind.lib()
     M, D, F, O = _sizes(x, wg, wd)
     n = _workspace_bytes(M, D, F, O, code, 0)
-    y = torch.empty((M, O), dtype=x.dtype, device=x.device)
+    y = x.new_empty((M, O))
     with _bind.on_device(x) as stream:
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(n, dtype=torch.uint8)
         _bind.check(lib.envidr_gated_mlp_forward(x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), wd.data_ptr(), wd.stride(0),
                                                  M, D, F, O, code, act, y.data_ptr(), O, ws.data_ptr(), n, stream), "envidr_gated_mlp_forward")
     return y
@@ -58,10 +59,10 @@ class _GatedMlp(torch.autograd.Function):
         M, D, F, O = _sizes(x, wg, wd)
         dy = _rows(dy)
         n = _workspace_bytes(M, D, F, O, ctx.code, 1)
-        grads = [torch.empty(shape, dtype=x.dtype, device=x.device) if want else None for want, shape in zip(ctx.needs_input_grad, ((M, D), (F, D), (F, D), (O, F)))]
+        grads = [x.new_empty(shape) if want else None for want, shape in zip(ctx.needs_input_grad, ((M, D), (F, D), (F, D), (O, F)))]
         at = [None if g is None else g.data_ptr() for g in grads]
         with _bind.on_device(x) as stream:
-            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+            ws = x.new_empty(n, dtype=torch.uint8)
             _bind.check(lib.envidr_gated_mlp_backward(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0),
                                                       wd.data_ptr(), wd.stride(0), M, D, F, O, ctx.code, ctx.act, at[0], D, at[1], at[2], at[3],
                                                       ws.data_ptr(), n, stream), "envidr_gated_mlp_backward")
@@ -82,12 +83,12 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
                                "x [..., D], w_gate and w_up [F, D], w_down [O, F] are wanted")
     if 0 in w_gate.shape or 0 in w_down.shape:
         raise _lib.EnvidrError("gated_mlp: a width is zero")
-    rows = _rows(x.reshape(-1, x.shape[-1]))
+    rows = _rows(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
         y = _GatedMlp.apply(rows, _rows(w_gate), _rows(w_up), _rows(w_down), code, ACTIVATIONS[activation])
     else:
         y = _forward(rows, _rows(w_gate), _rows(w_up), _rows(w_down), code, ACTIVATIONS[activation])
-    return y.reshape(*x.shape[:-1], y.shape[-1])
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 
 
 class GatedMLP(torch.nn.Module):

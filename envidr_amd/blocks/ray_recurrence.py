@@ -21,13 +21,12 @@ def _forward(gate, value, rays, state, code, blend, keep):
     lib = _bind.lib()
     T, C = gate.shape
     N = rays.shape[0]
-    device = gate.device
     n, n_saved = _sizes(T, N, C)
-    h = torch.empty((T, C), dtype=gate.dtype, device=device)
-    last = torch.empty((N, C), dtype=torch.float32, device=device)
-    saved = torch.empty(n_saved, dtype=torch.float32, device=device) if keep else None
+    h = torch.empty_like(gate)
+    last = gate.new_empty((N, C), dtype=torch.float32)
+    saved = gate.new_empty(n_saved, dtype=torch.float32) if keep else None
     with _bind.on_device(gate) as stream:
-        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        ws = gate.new_empty(n, dtype=torch.uint8)
         _bind.check(lib.envidr_ray_recurrence_forward(gate.data_ptr(), value.data_ptr(), rays.data_ptr(), None if state is None else state.data_ptr(), T, N, C, code, blend,
                                                       h.data_ptr(), last.data_ptr(), saved.data_ptr() if keep else None, ws.data_ptr(), n, stream),
                     "envidr_ray_recurrence_forward")
@@ -50,15 +49,14 @@ class _RayRecurrence(torch.autograd.Function):
         lib = _bind.lib()
         T, C = gate.shape
         N = rays.shape[0]
-        device = gate.device
         n = _sizes(T, N, C)[0]
-        dh = torch.zeros((T, C), dtype=gate.dtype, device=device) if dh is None else dh.contiguous()
+        dh = torch.zeros_like(gate) if dh is None else dh.contiguous()
         if dlast is not None:
             dlast = dlast.contiguous()
-        dgate, dvalue = (torch.empty((T, C), dtype=gate.dtype, device=device) for _ in range(2))
-        dstate = torch.empty((N, C), dtype=torch.float32, device=device) if ctx.needs_input_grad[2] else None
+        dgate, dvalue = torch.empty_like(gate), torch.empty_like(gate)
+        dstate = gate.new_empty((N, C), dtype=torch.float32) if ctx.needs_input_grad[2] else None
         with _bind.on_device(gate) as stream:
-            ws = torch.empty(n, dtype=torch.uint8, device=device)
+            ws = gate.new_empty(n, dtype=torch.uint8)
             _bind.check(lib.envidr_ray_recurrence_backward(dh.data_ptr(), None if dlast is None else dlast.data_ptr(), gate.data_ptr(), value.data_ptr(), rays.data_ptr(),
                                                            None if state is None else state.data_ptr(), saved.data_ptr(), T, N, C, ctx.code, ctx.blend,
                                                            dgate.data_ptr(), dvalue.data_ptr(), None if dstate is None else dstate.data_ptr(), ws.data_ptr(), n, stream),
