@@ -13,7 +13,8 @@
 // Operands that the core cannot read as they are (fp32: three bf16 terms; widths, pitches or addresses that are no multiples of 16 bytes) are
 // laid out first by k_pack_operands.  Rows go in chunks of at most kChunkBytes of hidden-layer operands.
 //
-// Narrow layers of the 16-bit types (all weights in one CU's LDS) go forward in one kernel (gated_narrow.hip).
+// Narrow layers of the 16-bit types go forward in one kernel (all weights in one CU's LDS: gated_narrow.hip) and backward in another (the sums of
+// the weights' gradients in one CU's registers: gated_narrow_grad.hip).
 //
 // Of few rows the weights' bytes are all there is to move: k_few_rows streams them once through registers, sixteen weight rows a workgroup, the
 // reduction split over its waves.
@@ -293,15 +294,27 @@ struct SumArgs {
     SumJob job[3];
     uint32_t jobs, splits;
 };
-template <class E> __global__ void __launch_bounds__(kBlock) k_sum_splits(SumArgs a) {
+// SHARE threads add up a result's parts, every SHARE-th each, and the first adds theirs
+template <class E, int SHARE> __global__ void __launch_bounds__(kBlock) k_sum_splits(SumArgs a) {
+    constexpr uint32_t kResults = kBlock / SHARE;
     uint32_t j = 0;
     while (j + 1 < a.jobs && blockIdx.x >= a.job[j + 1].first_block) ++j;
     const SumJob& s = a.job[j];
-    const uint64_t i = (uint64_t)(blockIdx.x - s.first_block) * kBlock + threadIdx.x;
-    if (i >= s.n) return;
+    const uint64_t i = (uint64_t)(blockIdx.x - s.first_block) * kResults + threadIdx.x % kResults;
     float v = 0;
-    for (uint32_t k = 0; k < a.splits; ++k) v += s.part[k * s.n + i];
-    static_cast<E*>(s.out)[(int64_t)(i / s.cols) * s.ld + (int64_t)(i % s.cols)] = from_f32<E>(v);
+    if (i < s.n) {
+#pragma unroll 8
+        for (uint32_t k = threadIdx.x / kResults; k < a.splits; k += SHARE) v += s.part[k * s.n + i];
+    }
+    if constexpr (SHARE > 1) {
+        __shared__ float shared[kBlock];
+        shared[threadIdx.x] = v;
+        __syncthreads();
+        if (threadIdx.x >= kResults) return;
+#pragma unroll
+        for (int k = 1; k < SHARE; ++k) v += shared[k * kResults + threadIdx.x];
+    }
+    if (i < s.n) static_cast<E*>(s.out)[(int64_t)(i / s.cols) * s.ld + (int64_t)(i % s.cols)] = from_f32<E>(v);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------------------------
@@ -472,6 +485,11 @@ Plan make_plan(uint32_t M, uint32_t D, uint32_t F, uint32_t O, int dtype, bool b
         p.bytes = 16;
         return p;
     }
+    if (backward && gated_grad_is_narrow(D, F, O, dtype)) {
+        p.splits = gated_narrow_grad_parts(M, D, F);
+        p.bytes = 4ull * p.splits * (2ull * F * D + (uint64_t)O * F);
+        return p;
+    }
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) { const uint64_t here = at; at += round_up64(bytes, 256); return here; };
     p.wg = take(2ull * p.np * F * p.Dp);
@@ -584,6 +602,34 @@ bool whole_units(const void* p, int64_t ld, uint32_t cols, uint32_t size) {
     const uint32_t unit = 16u / size;
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % unit == 0 && cols % unit == 0;
 }
+// adds up parts: `add` fills in where they lie and where their sums go
+struct Sums {
+    SumArgs a{};
+    uint32_t share, blocks = 0;
+    explicit Sums(uint32_t splits) {
+        a.splits = splits;
+        share = splits >= 32u ? 4u : 1u;             // @@
+    }
+    void add(const float* part, void* out, uint64_t rows, uint32_t cols, int64_t ld) {
+        const uint64_t n = rows * cols, results = kBlock / share;
+        a.job[a.jobs++] = {part, out, n, blocks, cols, ld};
+        blocks += (uint32_t)((n + results - 1) / results);
+    }
+    template <class E> int launch(hipStream_t s) {
+        if (share == 4u) hipLaunchKernelGGL((k_sum_splits<E, 4>), dim3(blocks), dim3(kBlock), 0, s, a);
+        else hipLaunchKernelGGL((k_sum_splits<E, 1>), dim3(blocks), dim3(kBlock), 0, s, a);
+        return check_launch("k_sum_splits");
+    }
+};
+// the weights' gradients from their parts, which lie one behind the other
+template <class E> int sum_weight_grads(const float* part, uint32_t splits, uint32_t D, uint32_t F, uint32_t O, void* dwg, void* dwu, void* dwd, hipStream_t s) {
+    const uint64_t fd = (uint64_t)splits * F * D;
+    Sums u(splits);
+    if (dwg) u.add(part, dwg, F, D, D);
+    if (dwu) u.add(part + fd, dwu, F, D, D);
+    if (dwd) u.add(part + 2 * fd, dwd, O, F, F);
+    return u.template launch<E>(s);
+}
 template <class E, bool BKC> int launch_product(ProductArgs a, const Plan& p, char* ws, hipStream_t s) {
     constexpr int NP = Terms<E>::NP;
     a.aligned = whole_units(a.out, a.ld, a.N, sizeof(E));
@@ -592,13 +638,9 @@ template <class E, bool BKC> int launch_product(ProductArgs a, const Plan& p, ch
         a.per_split = p.product_per_split;
         a.part = reinterpret_cast<float*>(ws + p.product_part);
         if (int rc = launch_product_as<E, 128, 128, 2, 2, BKC>(a, s)) return rc;
-        SumArgs u{};
-        u.jobs = 1;
-        u.splits = a.splits * a.phases;
-        const uint64_t n = (uint64_t)a.M * a.N;
-        u.job[0] = {a.part, a.out, n, 0, a.N, a.ld};
-        hipLaunchKernelGGL((k_sum_splits<E>), dim3((uint32_t)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, u);
-        return check_launch("k_sum_splits");
+        Sums u(a.splits * a.phases);
+        u.add(a.part, a.out, a.M, a.N, a.ld);
+        return u.template launch<E>(s);
     }
     if (!large_product(a.M, a.N, NP)) return launch_product_as<E, 128, 128, 2, 2, BKC>(a, s);
     if constexpr (NP == 1) return launch_product_as<E, 256, 256, 2, 4, BKC>(a, s);
@@ -710,6 +752,15 @@ template <class E> int backward(const void* dy, int64_t lddy, const void* x, int
     using T = typename Terms<E>::T;
     constexpr int NP = Terms<E>::NP;
     const Plan p = make_plan(M, D, F, O, dtype, true);
+    if constexpr (NP == 1) {
+        if (gated_grad_is_narrow(D, F, O, dtype)) {
+            float* parts = reinterpret_cast<float*>(ws);
+            const bool want_w = dwg || dwu || dwd;
+            if (!dx && !want_w) return ENVIDR_OK;
+            if (int rc = gated_narrow_backward({dy, x, w.wg, w.wu, w.wd, dx, parts, lddy, ldx, w.lg, w.lu, w.ldn, lddx, M, D, F, O, 0, want_w}, dtype, act, s)) return rc;
+            return want_w ? sum_weight_grads<E>(parts, p.splits, D, F, O, dwg, dwu, dwd, s) : ENVIDR_OK;
+        }
+    }
     Operand owg{}, owu{}, owd{};
     float* part = p.part ? reinterpret_cast<float*>(ws + p.part) : nullptr;
     auto strided = [](Operand o, uint32_t ext) { o.ext = ext; return o; };
@@ -765,23 +816,7 @@ template <class E> int backward(const void* dy, int64_t lddy, const void* x, int
             if (int rc = launch_weight_grads<E>(g, p.large_grads, s)) return rc;
         }
     }
-    if (part && (dwg || dwu || dwd)) {
-        SumArgs u{};
-        u.splits = p.splits;
-        uint32_t blocks = 0;
-        auto job = [&](void* out, uint64_t part_at, uint32_t n_rows, uint32_t n_cols) {
-            if (!out) return;
-            const uint64_t n = (uint64_t)n_rows * n_cols;
-            u.job[u.jobs++] = {part + part_at, out, n, blocks, n_cols, n_cols};
-            blocks += (uint32_t)((n + kBlock - 1) / kBlock);
-        };
-        const uint64_t fd = (uint64_t)p.splits * F * D;
-        job(dwg, 0, F, D);
-        job(dwu, fd, F, D);
-        job(dwd, 2 * fd, O, F);
-        hipLaunchKernelGGL((k_sum_splits<E>), dim3(blocks), dim3(kBlock), 0, s, u);
-        return check_launch("k_sum_splits");
-    }
+    if (part && (dwg || dwu || dwd)) return sum_weight_grads<E>(part, p.splits, D, F, O, dwg, dwu, dwd, s);
     return ENVIDR_OK;
 }
 

@@ -24,4 +24,18 @@ struct NarrowArgs {
 bool gated_is_narrow(uint32_t D, uint32_t F, uint32_t O, int dtype);
 int gated_narrow_forward(const NarrowArgs& a, int dtype, int activation, hipStream_t s);
 
+// their gradients: dx [M][D] or NULL; the weights' as `parts` partial sums in fp32, part = [parts][F][D] of the gate, the same of the up, [parts][O][F] of
+// the down matrix
+struct NarrowGradArgs {
+    const void *dy, *x, *wg, *wu, *wd;
+    void* dx;
+    float* part;
+    int64_t lddy, ldx, lg, lu, ldn, lddx;
+    uint32_t M, D, F, O, slices;    // slices: set by the launch
+    bool want_w;
+};
+bool gated_grad_is_narrow(uint32_t D, uint32_t F, uint32_t O, int dtype);
+uint32_t gated_narrow_grad_parts(uint32_t M, uint32_t D, uint32_t F);
+int gated_narrow_backward(NarrowGradArgs a, int dtype, int activation, hipStream_t s);
+
 }  // namespace envidr

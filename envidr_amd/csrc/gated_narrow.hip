@@ -27,20 +27,6 @@ __device__ __forceinline__ uint32_t narrow_swizzle(uint32_t units, uint32_t row)
     return p ^ ((units == 4u ? p ^ (p >> 1) : units == 8u ? (p >> 1) ^ (p >> 2) : (p >> 2) ^ (p >> 3)) & 1u);
 }
 
-// Eight adjacent elements from column k of a row of n; zeros behind it.  whole: n is a multiple of 8, and a load behind it is a load of the last
-// eight instead, made zero: no branch, so that loads can go out together.
-template <class E> __device__ __forceinline__ s16x8 load8(const E* row, uint32_t k, uint32_t n, bool whole) {
-    if (whole) {
-        const s16x8 v = __builtin_bit_cast(s16x8, load_pack<E, 8>(row + min(k, n - 8u)));
-        return k < n ? v : s16x8{};
-    }
-    if (k + 8u <= n) return __builtin_bit_cast(s16x8, load_pack<E, 8>(row + k));
-    Pack<E, 8> v;
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) v.v[i] = k + i < n ? row[k + i] : from_f32<E>(0.0f);
-    return __builtin_bit_cast(s16x8, v);
-}
-
 // KD: k blocks of 32 of the input width; OB: blocks of 16 of the output width
 template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(narrow_waves(KD, OB) * 64, narrow_waves(KD, OB) / 4) k_narrow_forward(NarrowArgs a) {
     constexpr int kNarrowWaves = narrow_waves(KD, OB);

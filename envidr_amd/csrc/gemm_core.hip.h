@@ -27,6 +27,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) s16x8 lds_s16x8;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
 struct Operand {
     const uint16_t* p;      // plane 0
@@ -469,5 +470,19 @@ template <class T, int NP, int COLS> struct PlaneStore {
         }
     }
 };
+
+// Eight adjacent elements from column k of a row of n; zeros behind it.  whole: n is a multiple of 8, and a load behind it is a load of the last
+// eight instead, made zero: no branch, so that loads can go out together.
+template <class E> __device__ __forceinline__ s16x8 load8(const E* row, uint32_t k, uint32_t n, bool whole) {
+    if (whole) {
+        const s16x8 v = __builtin_bit_cast(s16x8, load_pack<E, 8>(row + min(k, n - 8u)));
+        return k < n ? v : s16x8{};
+    }
+    if (k + 8u <= n) return __builtin_bit_cast(s16x8, load_pack<E, 8>(row + k));
+    Pack<E, 8> v;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v.v[i] = k + i < n ? row[k + i] : from_f32<E>(0.0f);
+    return __builtin_bit_cast(s16x8, v);
+}
 
 }  // namespace envidr

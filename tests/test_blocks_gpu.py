@@ -30,7 +30,9 @@ def _mlp_inputs(g, dt, M, D, F, O):
 MLP_SHAPES = [(1, 1, 1, 1), (1, 512, 2048, 512), (2, 72, 256, 12), (15, 7, 33, 5), (16, 250, 1000, 250), (17, 64, 128, 64), (33, 90, 300, 20), (63, 130, 70, 9), (64, 256, 520, 256), (65, 256, 520, 256), (127, 72, 256, 12),
               (128, 128, 128, 128), (129, 8, 16, 8), (300, 257, 131, 259), (1000, 39, 64, 3), (4097, 72, 264, 16), (20011, 40, 72, 24),
               (40, 456, 944, 144), (200, 90, 2001, 77),
-              (700, 128, 33, 64), (1000, 20, 900, 16), (33, 100, 250, 40)]
+              (700, 128, 33, 64), (1000, 20, 900, 16), (33, 100, 250, 40),
+              # narrow layers whose gradients' sums stay in registers: one to eight teams, the widest, and more rows than a round of workgroups takes
+              (31, 96, 256, 32), (33, 96, 250, 17), (300, 65, 40, 1), (257, 33, 20, 17), (1031, 64, 100, 1), (600, 1, 64, 32), (20000, 24, 200, 8), (70000, 5, 30, 4)]
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=str)
