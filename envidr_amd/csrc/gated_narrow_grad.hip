@@ -7,12 +7,14 @@
 //      16 + 4 q + 3} (q = lane / 16) are one 16-byte unit there, so units lie in that order;
 //   2. dWg += dg^T x, dWu += du^T x, dWd += dy^T h: the reduction over the rows is one k step of the matrix core; both operands are transposing
 //      reads, of columns that the wave wrote itself, the sums stay in registers from the first row to the last;
-//   3. behind a barrier, since a team's waves need each other's units: dx = dg Wg + du Wu, a block of 16 columns a wave, the weights from LDS.
-// Next rows are loaded under the present ones' work and put into LDS beside step 3.  At the end the teams' sums are added up in LDS and the
+//   3. behind a barrier, since a team's waves need each other's units: dx = dg Wg + du Wu, a block of 16 columns a wave, the weights from LDS; the
+//      results go through x's place in LDS, so that rows are written whole (10^6 rows of 32 -> 64 -> 12: 127 us; in blocks of 16 columns 145).
+// Next rows are loaded under the present ones' work and follow dx there.  At the end the teams' sums are added up in LDS and the
 // workgroup's go to `part`; k_sum_splits adds those of all workgroups, in order.
 // LDS rows are an odd multiple of 32 bytes apart: sixteen-byte reads of sixteen rows and transposing reads of eight rows both find them on
 // different banks (for the transposing ones the rows of a k step are taken as 4 q .. 4 q + 3, 16 + 4 q .. 16 + 4 q + 3).
-// Bound: the vector ALU (the activation and its slope), then LDS.  @@
+// Bound: the phases' latencies with two waves a SIMD (the sums take half the registers): vector ALU 35 %, LDS 26 %, matrix cores 20 % busy.
+// 146 000 rows of 72 -> 256 -> 12 in bf16: 93 us and 8 for the parts; through memory (hidden layer's operands, products, transposed products) 198.
 #include "gated_mlp.hip.h"
 #include "gemm_core.hip.h"
 
@@ -31,9 +33,12 @@ __device__ __forceinline__ s16x8 columns(uint32_t at, uint32_t pitch, uint32_t l
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// KD: k blocks of 32 of the input width; ONE: one team, whose rows are one 16-byte unit a thread at most
-template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(kWaves * 64, 2) k_narrow_backward(NarrowGradArgs a) {
-    constexpr int DB = 2 * KD;                                                   // blocks of 16 input columns
+// everyone's LDS operations are done.  (__syncthreads would wait for memory too: for dx to be written and the next rows to be read)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// DB: blocks of 16 input columns; ONE: one team, whose rows are one 16-byte unit a thread at most
+template <class E, int ACT, int DB, bool ONE> __global__ void __launch_bounds__(kWaves * 64, 2) k_narrow_backward(NarrowGradArgs a) {
+    constexpr int KD = (DB + 1) / 2;                                             // k blocks of 32 of them
     constexpr uint32_t kXPitch = KD * 64 + 32;
     constexpr int kXUnits = ONE ? 1 : 2 * KD, kDyUnits = ONE ? 1 : 2;            // 16-byte units a thread carries, at most
     __shared__ __attribute__((aligned(1024))) char lds_all[kLds];
@@ -46,6 +51,7 @@ template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(
     const bool whole_x = a.D % 8u == 0u, whole_y = a.O % 8u == 0u;
     const uint32_t rows = teams * kTeamRows, tiles = (a.M + rows - 1u) / rows;
 
+    auto x_unit = [&](uint32_t n) { return teams_at + n / (KD * 4u) / kTeamRows * team_bytes + n / (KD * 4u) % kTeamRows * kXPitch + n % (KD * 4u) * 16u; };
     // the next rows of x and dy, and where they go: unit n of a tile is row n / units, zeros behind the last row and column
     s16x8 nx[kXUnits], ny[kDyUnits];
     auto fetch = [&](uint32_t t) {
@@ -64,12 +70,29 @@ template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(
 #pragma unroll
         for (int j = 0; j < kXUnits; ++j) {
             const uint32_t n = j * (kWaves * 64u) + threadIdx.x, r = n / (KD * 4u);
-            if (r < rows) *(lds_s16x8*)(teams_at + r / kTeamRows * team_bytes + r % kTeamRows * kXPitch + n % (KD * 4u) * 16u) = nx[j];
+            if (r < rows) *(lds_s16x8*)(x_unit(n)) = nx[j];
         }
 #pragma unroll
         for (int j = 0; j < kDyUnits; ++j) {
             const uint32_t n = j * (kWaves * 64u) + threadIdx.x, r = n / 4u;
             if (r < rows) *(lds_s16x8*)(teams_at + r / kTeamRows * team_bytes + kTeamRows * kXPitch + r % kTeamRows * kDyPitch + n % 4u * 16u) = ny[j];
+        }
+    };
+    // dx of tile t, which has taken x's place in LDS: whole rows, the units that this thread puts the next x into
+    auto store_dx = [&](uint32_t t) {
+#pragma unroll
+        for (int j = 0; j < kXUnits; ++j) {
+            const uint32_t n = j * (kWaves * 64u) + threadIdx.x, r = n / (KD * 4u), c = n % (KD * 4u) * 8u, m = t * rows + r;
+            if (r >= rows || m >= a.M || c >= a.D) continue;
+            const Pack<E, 8> v = __builtin_bit_cast(Pack<E, 8>, *(const lds_s16x8*)(x_unit(n)));
+            E* to = static_cast<E*>(a.dx) + (int64_t)m * a.lddx + c;
+            if (a.D - c >= 8u) {
+                store_pack(to, v);
+            } else {
+#pragma unroll
+                for (uint32_t q = 0; q < 7; ++q)
+                    if (c + q < a.D) to[q] = v.v[q];
+            }
         }
     };
     uint32_t t = blockIdx.x;                                                     // (the grid has no more workgroups than tiles)
@@ -104,8 +127,8 @@ template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(
             for (int rb = 0; rb < 2; ++rb) dh[rb] = mfma16<E>(rd[b], *(const lds_s16x8*)(ys + (rb * 16u + i) * kDyPitch + g * 16u), f32x4{});
 #pragma unroll
             for (int kk = 0; kk < KD; ++kk) {
-                const uint32_t at = (slice * 32u + b * 16u + i) * kXPitch + (kk * 4u + g) * 16u;
-                const s16x8 w = *(const lds_s16x8*)(lds_w + at), v = *(const lds_s16x8*)(lds_w + hidden * kXPitch + at);
+                const uint32_t at = lds_w + (slice * 32u + b * 16u + i) * kXPitch + (kk * 4u + g) * 16u;
+                const s16x8 w = *(const lds_s16x8*)at, v = *(const lds_s16x8*)(at + hidden * kXPitch);
 #pragma unroll
                 for (int rb = 0; rb < 2; ++rb) {
                     const s16x8 x = *(const lds_s16x8*)(xs + (rb * 16u + i) * kXPitch + (kk * 4u + g) * 16u);
@@ -114,7 +137,7 @@ template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(
                 }
             }
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
+            for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     float act, slope;
@@ -123,7 +146,6 @@ template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(
                     vg[rb].v[4 * b + q] = from_f32<E>(dh[rb][q] * pu[rb][q] * slope);
                     vu[rb].v[4 * b + q] = from_f32<E>(dh[rb][q] * act);
                 }
-            }
         }
         s16x8 du[2];
 #pragma unroll
@@ -137,15 +159,12 @@ template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(
         }
         // (LDS operations of a wave are done in their order; the compiler has to leave them in it: lanes read what others wrote)
         asm volatile("" ::: "memory");
+        s16x8 h[2], ty[2];
         if (a.want_w) {
-            s16x8 h[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) h[c] = columns(dus + slice * 64u + c * 32u, h_pitch, lane);
-#pragma unroll
-            for (int o = 0; o < 2; ++o) {
-                const s16x8 y = columns(ys + o * 32u, kDyPitch, lane);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) sum_d[c][o] = mfma16<E>(h[c], y, sum_d[c][o]);
+            for (int c = 0; c < 2; ++c) {
+                h[c] = columns(dus + slice * 64u + c * 32u, h_pitch, lane);
+                ty[c] = columns(ys + c * 32u, kDyPitch, lane);
             }
         }
         asm volatile("" ::: "memory");
@@ -153,51 +172,78 @@ template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(
         for (int rb = 0; rb < 2; ++rb) *(lds_s16x8*)(dus + (rb * 16u + i) * h_pitch + (slice * 4u + g) * 16u) = du[rb];
         asm volatile("" ::: "memory");
         if (a.want_w) {
-            s16x8 tg[2], tu[2];
+            s16x8 tg[2], tu[2], tx[DB];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 tg[c] = columns(dgs + slice * 64u + c * 32u, h_pitch, lane);
                 tu[c] = columns(dus + slice * 64u + c * 32u, h_pitch, lane);
             }
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const s16x8 x = columns(xs + d * 32u, kXPitch, lane);
+            for (int d = 0; d < DB; ++d) tx[d] = columns(xs + d * 32u, kXPitch, lane);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    sum_g[c][d] = mfma16<E>(x, tg[c], sum_g[c][d]);
-                    sum_u[c][d] = mfma16<E>(x, tu[c], sum_u[c][d]);
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int o = 0; o < 2; ++o) sum_d[c][o] = mfma16<E>(h[c], ty[o], sum_d[c][o]);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    sum_g[c][d] = mfma16<E>(tx[d], tg[c], sum_g[c][d]);
+                    sum_u[c][d] = mfma16<E>(tx[d], tu[c], sum_u[c][d]);
                 }
             }
         }
-        __syncthreads();
+        lds_barrier();
         if (a.dx) {
-            const uint32_t m0 = t * rows + team * kTeamRows;
 #pragma unroll 1
             for (uint32_t d = slice; d < blocks; d += slices) {
                 f32x4 p[2][2] = {};
-#pragma unroll 1
-                for (uint32_t hb = 0; hb < slices; ++hb) {
-                    const s16x8 ng = columns(lds_w + hb * 32u * kXPitch + d * 32u, kXPitch, lane), nu = columns(lds_w + (hidden + hb * 32u) * kXPitch + d * 32u, kXPitch, lane);
+                // (the next units' reads under the present ones' products)
+                struct Units {
+                    s16x8 w[2], h[2][2];
+                } now, next;
+                auto read = [&](Units& u, uint32_t hb) {
+                    u.w[0] = columns(lds_w + hb * 32u * kXPitch + d * 32u, kXPitch, lane);
+                    u.w[1] = columns(lds_w + (hidden + hb * 32u) * kXPitch + d * 32u, kXPitch, lane);
 #pragma unroll
                     for (int rb = 0; rb < 2; ++rb) {
                         const uint32_t at = (rb * 16u + i) * h_pitch + (hb * 4u + g) * 16u;
-                        p[0][rb] = mfma16<E>(ng, *(const lds_s16x8*)(dgs + at), p[0][rb]);
-                        p[1][rb] = mfma16<E>(nu, *(const lds_s16x8*)(dus + at), p[1][rb]);
+                        u.h[0][rb] = *(const lds_s16x8*)(dgs + at);
+                        u.h[1][rb] = *(const lds_s16x8*)(dus + at);
+                    }
+                };
+                auto multiply = [&](const Units& u) {
+#pragma unroll
+                    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) p[m][rb] = mfma16<E>(u.w[m], u.h[m][rb], p[m][rb]);
+                };
+                if constexpr (ONE) {
+                    read(now, 0);
+#pragma unroll 1
+                    for (uint32_t hb = 0; hb < slices; hb += 2) {
+                        read(next, hb + 1);
+                        multiply(now);
+                        if (hb + 2 < slices) read(now, hb + 2);
+                        multiply(next);
+                    }
+                } else {                     // (two sets of operands and several teams' rows would not fit the registers)
+#pragma unroll 1
+                    for (uint32_t hb = 0; hb < slices; ++hb) {
+                        read(now, hb);
+                        multiply(now);
                     }
                 }
 #pragma unroll
                 for (int rb = 0; rb < 2; ++rb) {
-                    const uint32_t m = m0 + rb * 16u + i, n = d * 16u + 4u * g;
-                    if (m >= a.M) continue;
-                    const f32x4 s = p[0][rb] + p[1][rb];
-                    const float v[4] = {s[0], s[1], s[2], s[3]};
-                    store_row4(static_cast<E*>(a.dx) + (int64_t)m * a.lddx + n, (int64_t)a.D - n, v);
+                    const f32x4 v = p[0][rb] + p[1][rb];
+                    *(lds_s16x4*)(xs + (rb * 16u + i) * kXPitch + d * 32u + g * 8u) = pack4<E>({v[0], v[1], v[2], v[3]});
                 }
             }
+            lds_barrier();
+            store_dx(t);
         }
         if (!more) break;
         put();
-        __syncthreads();
+        lds_barrier();
         t += gridDim.x;
     }
     if (!a.want_w) return;
@@ -248,16 +294,15 @@ template <class E, int ACT, int KD, bool ONE> __global__ void __launch_bounds__(
 }
 
 template <class E, int ACT> int launch(const NarrowGradArgs& a, uint32_t grid, hipStream_t s) {
-    auto go = [&](auto kd, auto one) { hipLaunchKernelGGL((k_narrow_backward<E, ACT, decltype(kd)::value, decltype(one)::value>), dim3(grid), dim3(kWaves * 64), 0, s, a); };
-    auto with_kd = [&](auto kd) {
-        if (a.slices == kWaves) go(kd, std::true_type{});
-        else go(kd, std::false_type{});
+    auto go = [&](auto db, auto one) { hipLaunchKernelGGL((k_narrow_backward<E, ACT, decltype(db)::value, decltype(one)::value>), dim3(grid), dim3(kWaves * 64), 0, s, a); };
+    auto any = [&](auto db) {
+        if (a.slices == kWaves) go(db, std::true_type{});
+        else go(db, std::false_type{});
     };
-    switch (ceil_div(a.D, 32u)) {
-        case 1: with_kd(std::integral_constant<int, 1>{}); break;
-        case 2: with_kd(std::integral_constant<int, 2>{}); break;
-        default: go(std::integral_constant<int, 3>{}, std::true_type{}); break;
-    }
+    if (a.D <= 32u) any(std::integral_constant<int, 2>{});
+    else if (a.D <= 64u) any(std::integral_constant<int, 4>{});
+    else if (a.D <= 80u) go(std::integral_constant<int, 5>{}, std::true_type{});
+    else go(std::integral_constant<int, 6>{}, std::true_type{});
     return check_launch("k_narrow_backward");
 }
 
@@ -271,6 +316,8 @@ uint32_t slices_of(uint32_t D, uint32_t F) {
 
 }  // namespace
 
+// Widths whose gradients' sums fit eight waves' registers.  Against the tiles, a training pass in bf16: 146 000 rows of 72 -> 256 -> 12 245 -> 131 us, of 96 -> 33
+// -> 32 141 -> 111, of 32 -> 64 -> 16 126 -> 45; 10 000 rows of 72 -> 256 -> 12 51 both; 65 rows 35 -> 32.
 bool gated_grad_is_narrow(uint32_t D, uint32_t F, uint32_t O, int dtype) { return dtype != ENVIDR_F32 && D <= 96 && F <= 256 && O <= 32; }
 
 uint32_t gated_narrow_grad_parts(uint32_t M, uint32_t D, uint32_t F) {
