@@ -13,8 +13,8 @@
 // Operands that the core cannot read as they are (fp32: three bf16 terms; widths, pitches or addresses that are no multiples of 16 bytes) are
 // laid out first by k_pack_operands.  Rows go in chunks of at most kChunkBytes of hidden-layer operands.
 //
-// Narrow layers of the 16-bit types go forward in one kernel (all weights in one CU's LDS: gated_narrow.hip) and backward in another (the sums of
-// the weights' gradients in one CU's registers: gated_narrow_grad.hip).
+// Narrow layers go forward in one kernel (all weights in one CU's LDS: gated_narrow.hip; fp32: in its registers, gated_narrow_fp32.hip), those of the
+// 16-bit types backward in another (the sums of the weights' gradients in one CU's registers: gated_narrow_grad.hip).
 //
 // Of few rows the weights' bytes are all there is to move: k_few_rows streams them once through registers, sixteen weight rows a workgroup, the
 // reduction split over its waves.
@@ -715,11 +715,7 @@ template <class E> int forward(const void* x, int64_t ldx, const Weights& w, uin
             if (M > 32) return go(std::integral_constant<int, 4>{});
         return go(std::integral_constant<int, 2>{});
     }
-    if constexpr (NP == 1) {
-        if (gated_is_narrow(D, F, O, dtype)) {
-            return gated_narrow_forward({x, w.wg, w.wu, w.wd, y, ldx, w.lg, w.lu, w.ldn, ldy, M, D, F, O}, dtype, act, s);
-        }
-    }
+    if (gated_is_narrow(D, F, O, dtype)) return gated_narrow_forward({x, w.wg, w.wu, w.wd, y, ldx, w.lg, w.lu, w.ldn, ldy, M, D, F, O}, dtype, act, s);
     Operand owg{}, owu{}, owd{};
     for (uint32_t m0 = 0; m0 < M; m0 += p.chunk) {
         const uint32_t rows = M - m0 < p.chunk ? M - m0 : p.chunk;

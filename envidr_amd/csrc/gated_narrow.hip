@@ -151,12 +151,14 @@ template <class E, int ACT> int launch_narrow(const NarrowArgs& a, hipStream_t s
 }  // namespace
 
 bool gated_is_narrow(uint32_t D, uint32_t F, uint32_t O, int dtype) {
-    if (dtype == ENVIDR_F32 || D > 128 || O > 64 || F > 4096) return false;
+    if (dtype == ENVIDR_F32) return D <= 96 && F <= 256 && O <= 32;              // (the weights' three terms in eight waves' registers)
+    if (D > 128 || O > 64 || F > 4096) return false;
     const uint32_t hidden = (F + 31u) / 32u * 32u;
     return 2u * hidden * narrow_units((D + 31u) / 32u) * 16u + (O <= 16u ? 16u : 64u) * narrow_down_units(hidden) * 16u <= (uint32_t)kNarrowLds;
 }
 
 int gated_narrow_forward(const NarrowArgs& a, int dtype, int activation, hipStream_t s) {
+    if (dtype == ENVIDR_F32) return gated_narrow_forward_fp32(a, activation, s);
     if (dtype == ENVIDR_BF16) ENVIDR_FOR_ACT(activation, ACT, return (launch_narrow<__bf16, ACT>(a, s)));
     ENVIDR_FOR_ACT(activation, ACT, return (launch_narrow<_Float16, ACT>(a, s)));
 }

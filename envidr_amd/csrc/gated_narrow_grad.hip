@@ -23,7 +23,7 @@
 namespace envidr {
 namespace {
 
-constexpr int kLds = 160 * 1024, kWaves = 8, kTeamRows = 32;
+constexpr int kLds = 160 * 1024, kWaves = kTeamWaves, kTeamRows = 32;
 constexpr uint32_t kDyPitch = 96;
 
 // an operand of sixteen columns and 32 rows (k) from `at`: rows 4 q .. and 16 + 4 q .. of the lane groups q
@@ -32,9 +32,6 @@ __device__ __forceinline__ s16x8 columns(uint32_t at, uint32_t pitch, uint32_t l
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16u * pitch));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-
-// everyone's LDS operations are done.  (__syncthreads would wait for memory too: for dx to be written and the next rows to be read)
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // DB: blocks of 16 input columns; ONE: one team, whose rows are one 16-byte unit a thread at most
 template <class E, int ACT, int DB, bool ONE> __global__ void __launch_bounds__(kWaves * 64, 2) k_narrow_backward(NarrowGradArgs a) {
@@ -306,14 +303,6 @@ template <class E, int ACT> int launch(const NarrowGradArgs& a, uint32_t grid, h
     return check_launch("k_narrow_backward");
 }
 
-// waves that share a team's rows: a power of two; all of them from 65 input columns on, where several teams' rows on their way do not fit the registers
-uint32_t slices_of(uint32_t D, uint32_t F) {
-    if (D > 64u) return kWaves;
-    uint32_t s = 1;
-    while (s * 32u < F) s *= 2u;
-    return s;
-}
-
 }  // namespace
 
 // Widths whose gradients' sums fit eight waves' registers.  Against the tiles, a training pass in bf16: 146 000 rows of 72 -> 256 -> 12 245 -> 131 us, of 96 -> 33
@@ -321,12 +310,12 @@ uint32_t slices_of(uint32_t D, uint32_t F) {
 bool gated_grad_is_narrow(uint32_t D, uint32_t F, uint32_t O, int dtype) { return dtype != ENVIDR_F32 && D <= 96 && F <= 256 && O <= 32; }
 
 uint32_t gated_narrow_grad_parts(uint32_t M, uint32_t D, uint32_t F) {
-    const uint32_t tiles = ceil_div(M, kWaves / slices_of(D, F) * (uint32_t)kTeamRows);
+    const uint32_t tiles = ceil_div(M, kWaves / narrow_slices(D, F) * (uint32_t)kTeamRows);
     return tiles < 256u ? tiles : 256u;
 }
 
 int gated_narrow_backward(NarrowGradArgs a, int dtype, int activation, hipStream_t s) {
-    a.slices = slices_of(a.D, a.F);
+    a.slices = narrow_slices(a.D, a.F);
     const uint32_t grid = gated_narrow_grad_parts(a.M, a.D, a.F);
     if (dtype == ENVIDR_BF16) ENVIDR_FOR_ACT(activation, ACT, return (launch<__bf16, ACT>(a, grid, s)));
     ENVIDR_FOR_ACT(activation, ACT, return (launch<_Float16, ACT>(a, grid, s)));

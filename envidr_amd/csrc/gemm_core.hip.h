@@ -146,6 +146,9 @@ template <int TR, int KT, int NP, bool KC, int WAVES, bool PAIR = false> struct 
 // At most N of this wave's LDS-direct loads are still in flight, every LDS read of it is done, and so for the whole workgroup
 template <int N> __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
+// Every LDS operation of the workgroup is done.  (__syncthreads would wait for memory too)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // A workgroup's K loop over one pair of operands: acc[mi][ni] += A rows x B rows.  Wave (wm, wn) of WM x WN owns 16 MI x 16 NI of the tile.
 // Memory -> LDS: S stages of KT, S steps ahead; LDS -> registers: 32 k ahead, so that the reads run under the products of the 32 before
 // (the waves of a workgroup pass the barrier together: without this they would all read, then all multiply).
