@@ -6,7 +6,9 @@
 // holds units 4 q .. 4 q + 3 and 16 + 4 q .. 16 + 4 q + 3 of its row (q = lane / 16), which is one operand of the second product, in an order of k
 // that the lanes' parts of Wd follow.  So a wave forms its units' share of y by itself; the shares meet in LDS and are added up in the order of the
 // units.
-// Bound: matrix cores and vector ALU about alike (six products; the activation and the terms of h).  @@
+// Bound: matrix cores (six products a product: about 45 % of the time) and vector ALU (activation, terms of h: 40 %), which the two waves of a SIMD
+// use in turns.  146 000 rows of 72 -> 256 -> 12: 100 us (operands laid out and the hidden layer through memory: 232); of 32 -> 64 -> 16 31 (71);
+// 65 rows 18 (30).
 #include "gated_mlp.hip.h"
 #include "gemm_core.hip.h"
 
@@ -134,7 +136,8 @@ template <int ACT, int KD, bool ONE> __global__ void __launch_bounds__(kWaves * 
                 for (int q = 0; q < 4; ++q) h[4 * b + q] = activation_value<ACT, true>(pg[b][q]) * pu[b][q];
             const Terms8 s = split8(h);
 #pragma unroll
-            for (int o = 0; o < kOut; ++o) *(lds_f32x4*)(lds + ((wave * 2u + rb) * kOut + o) * 1024u + lane * 16u) = six(rd[o], s, f32x4{});
+            for (int o = 0; o < kOut; ++o)
+                if (o == 0 || a.O > 16u) *(lds_f32x4*)(lds + ((wave * 2u + rb) * kOut + o) * 1024u + lane * 16u) = six(rd[o], s, f32x4{});
         }
         lds_barrier();
         // the shares: unit n is (team, rows, columns, lane)'s four columns
