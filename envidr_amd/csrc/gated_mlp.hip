@@ -336,7 +336,7 @@ template <class E, int ACT, bool GLU, int MT> __global__ void __launch_bounds__(
     constexpr uint32_t kStep = 4 * W;                    // k of a wave's step: four lane groups
     constexpr int kMats = GLU ? 2 : 1;
     __shared__ f32x4 part[kMats][kFewWaves][64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15u, n0 = blockIdx.x * 16u;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15u, n0 = blockIdx.x * 16u;
     const A* a[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) a[t] = static_cast<const A*>(f.a) + (int64_t)min(16u * t + i, f.M - 1u) * f.lda;
@@ -353,34 +353,51 @@ template <class E, int ACT, bool GLU, int MT> __global__ void __launch_bounds__(
         for (int q = 0; q < W; ++q) v.v[q] = k + q < f.K ? p[k + q] : from_f32<P>(0.0f);
         return v;
     };
-    for (uint32_t k0 = wave * kStep; k0 < f.K; k0 += kFewWaves * kStep) {
-        const uint32_t k = k0 + g * W;
-        Pack<E, W> y[kMats];
-        Pack<A, W> x[MT];
+    // kAhead of a wave's steps at a time: their loads are all out before the first is waited for (one row, 1024 -> 4096 -> 1024: bf16 18 us, fp32 26;
+    // a step at a time 20 and 31)
+    constexpr int kAhead = MT == 1 ? 4 : 2;
+    for (uint32_t first = wave * kStep; first < f.K; first += kAhead * kFewWaves * kStep) {
+        Pack<E, W> y[kAhead][kMats];
+        Pack<A, W> x[kAhead][MT];
 #pragma unroll
-        for (int m = 0; m < kMats; ++m) y[m] = fetch(w[m], k);
+        for (int s = 0; s < kAhead; ++s) {
+            const uint32_t k0 = first + s * (kFewWaves * kStep), k = k0 + g * W;
+            if (k0 + kStep <= f.K) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) x[t] = fetch(a[t], k);
+                for (int m = 0; m < kMats; ++m) y[s][m] = load_pack<E, W>(w[m] + k);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            if constexpr (sizeof(E) == 4) {
+                for (int t = 0; t < MT; ++t) x[s][t] = load_pack<A, W>(a[t] + k);
+            } else if (k0 < f.K) {
 #pragma unroll
-                for (int m = 0; m < kMats; ++m)
+                for (int m = 0; m < kMats; ++m) y[s][m] = fetch(w[m], k);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[m].v[q], x[t].v[q], acc[m][t], 0, 0, 0);
-            } else if constexpr (GLU) {
+                for (int t = 0; t < MT; ++t) x[s][t] = fetch(a[t], k);
+            }
+        }
 #pragma unroll
-                for (int m = 0; m < kMats; ++m) acc[m][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[m]), __builtin_bit_cast(s16x8, x[t]), acc[m][t]);
-            } else {
-                Pack<E, W> hi, lo;
+        for (int s = 0; s < kAhead; ++s) {
+            if (first + s * (kFewWaves * kStep) >= f.K) break;
 #pragma unroll
-                for (int q = 0; q < W; ++q) {
-                    hi.v[q] = from_f32<E>(x[t].v[q]);
-                    const float rounded = to_f32(hi.v[q]);
-                    lo.v[q] = from_f32<E>(__builtin_isinf(rounded) ? 0.0f : x[t].v[q] - rounded);       // (inf - inf would be NaN)
+            for (int t = 0; t < MT; ++t) {
+                if constexpr (sizeof(E) == 4) {
+#pragma unroll
+                    for (int m = 0; m < kMats; ++m)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[s][m].v[q], x[s][t].v[q], acc[m][t], 0, 0, 0);
+                } else if constexpr (GLU) {
+#pragma unroll
+                    for (int m = 0; m < kMats; ++m) acc[m][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[s][m]), __builtin_bit_cast(s16x8, x[s][t]), acc[m][t]);
+                } else {
+                    Pack<E, W> hi, lo;
+#pragma unroll
+                    for (int q = 0; q < W; ++q) {
+                        hi.v[q] = from_f32<E>(x[s][t].v[q]);
+                        const float rounded = to_f32(hi.v[q]);
+                        lo.v[q] = from_f32<E>(__builtin_isinf(rounded) ? 0.0f : x[s][t].v[q] - rounded);       // (inf - inf would be NaN)
+                    }
+                    acc[0][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[s][0]), __builtin_bit_cast(s16x8, lo), acc[0][t]);
+                    acc[0][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[s][0]), __builtin_bit_cast(s16x8, hi), acc[0][t]);
                 }
-                acc[0][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[0]), __builtin_bit_cast(s16x8, lo), acc[0][t]);
-                acc[0][t] = mfma16<E>(__builtin_bit_cast(s16x8, y[0]), __builtin_bit_cast(s16x8, hi), acc[0][t]);
             }
         }
     }
