@@ -1,8 +1,8 @@
 // The gated feed-forward block of narrow layers, backward (16-bit types): dx, dWg, dWu and dWd in one pass over the rows, nothing of the hidden
 // layer through memory.
 //
-// A workgroup's eight waves form teams of `slices` waves; a team takes 32 rows at a time, a wave 32 hidden units of them, whose weights it keeps
-// in registers.  Per 32 rows:
+// A workgroup's eight waves form teams of `slices` waves; a team takes 32 rows at a time, a wave 32 hidden units of them.  The gate and up matrices
+// lie in LDS (in registers the sums of their gradients leave no room for them).  Per 32 rows:
 //   1. g, u, dh (x and dy from LDS) -> h, dg, du, rounded to the type, into LDS as [row][unit]; a lane's eight units {4 q .. 4 q + 3, 16 + 4 q ..
 //      16 + 4 q + 3} (q = lane / 16) are one 16-byte unit there, so units lie in that order;
 //   2. dWg += dg^T x, dWu += du^T x, dWd += dy^T h: the reduction over the rows is one k step of the matrix core; both operands are transposing
