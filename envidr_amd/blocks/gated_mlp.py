@@ -17,7 +17,9 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     pitch, step = t.stride()
     if step == 1 and t.shape[1] <= pitch <= 1 << 21:
         return t
-    return t.reshape(-1).view(t.shape)          # (contiguous() would leave a matrix of one row its pitch, whatever that is)
+    # contiguous() makes the elements adjacent (reshape alone would not: a matrix whose strides merge, t[:, ::2], is a view as one row too), but
+    # leaves a matrix of one row its pitch, whatever that is; the two views put it right
+    return t.contiguous().reshape(-1).view(t.shape)
 
 
 def _sizes(x, wg, wd):
