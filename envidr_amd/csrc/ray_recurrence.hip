@@ -226,8 +226,15 @@ template <int V> __device__ __forceinline__ void load_state(const float* s, int3
     for (int i = 0; i < V; ++i) h[i] = 0.0f;
 }
 
-template <bool BLEND> __device__ __forceinline__ float step(float h, float a, float an, float v) {
-    return BLEND ? fmaf(an, v - h, h) : fmaf(a, h, v);
+// One step.  Blend: a h + (1 - a) v, formed as (1 - w) near + w far with w the smaller weight and `near` what it leaves most of: an open gate (a
+// near 1, whose rounding would be all of 1 - a) goes by 1 - a, a closed one by a, and every rounding is one of a |h| or (1 - a) |v|.  (As
+// h + (1 - a) (v - h) a closed gate would leave 2^-24 of the h that it replaces.)  near's own infinity must not meet itself: w times the largest number
+// taken from it leaves it.
+template <bool BLEND> __device__ __forceinline__ float step(float gate, float h, float a, float an, float v) {
+    if constexpr (!BLEND) return fmaf(a, h, v);
+    const bool closed = gate < 0.0f;
+    const float w = closed ? a : an, near = closed ? v : h, far = closed ? h : v;
+    return fmaf(w, far, fmaf(-w, __builtin_amdgcn_fmed3f(near, -3.402823466e38f, 3.402823466e38f), near));
 }
 
 // Affine maps in order: first, then second.  A map that forgets its input -- a border of nobody, or the first border of a ray, which has the ray's
@@ -276,7 +283,7 @@ template <class E, int V, bool BLEND, bool UNI> __global__ void __launch_bounds_
                 for (int i = 0; i < V; ++i) {
                     float s, sn;
                     sigmoid_pair<sizeof(E) == 4>(x.g.at(j, i), s, sn);
-                    h[i] = step<BLEND>(h[i], s, sn, x.v.at(j, i));
+                    h[i] = step<BLEND>(x.g.at(j, i), h[i], s, sn, x.v.at(j, i));
                 }
                 store_row<E, V>(a.out0, row, a.C, p.c, h);
             }
@@ -328,7 +335,7 @@ template <class E, int V, bool BLEND, bool UNI> __global__ void __launch_bounds_
                     before[j][i] = x.h[i];
                     float s, sn;
                     sigmoid_pair<sizeof(E) == 4>(x.g.at(j, i), s, sn);
-                    const float then = step<BLEND>(x.h[i], s, sn, x.v.at(j, i));
+                    const float then = step<BLEND>(x.g.at(j, i), x.h[i], s, sn, x.v.at(j, i));
                     x.h[i] = row >= p.begin ? then : x.h[i];
                 }
             }
@@ -396,7 +403,7 @@ template <class E, int V, bool BLEND, bool BACK, bool UNI> __global__ void __lau
                 float s, sn;
                 sigmoid_pair<sizeof(E) == 4>(x.g.at(j, i), s, sn);
                 const float y = x.v.at(j, i);
-                B[i] = BACK ? s * (B[i] + y) : step<BLEND>(B[i], s, sn, y);
+                B[i] = BACK ? s * (B[i] + y) : step<BLEND>(x.g.at(j, i), B[i], s, sn, y);
                 A[i] *= s;
             }
         }
