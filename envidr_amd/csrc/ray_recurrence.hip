@@ -242,7 +242,11 @@ template <bool BLEND> __device__ __forceinline__ float step(float gate, float h,
 // small is +0 and forgets nothing: a NaN stays one along its own ray.)  The mark outlives a product with a later positive A.
 constexpr float kForget = -0.0f;
 __device__ __forceinline__ bool forgets(float A) { return __builtin_bit_cast(uint32_t, A) == 0x80000000u; }
-__device__ __forceinline__ float apply(float A, float B, float in) { return forgets(A) ? B : fmaf(A, in, B); }
+// That +0 is a number above zero, and an infinity times it is one.
+__device__ __forceinline__ float apply(float A, float B, float in) {
+    if (forgets(A)) return B;
+    return A == 0.0f && __builtin_isinf(in) ? in + B : fmaf(A, in, B);
+}
 
 // the state that crosses border k (forward: h before its row; backward: E behind the row before it)
 template <int V> __device__ __forceinline__ void load_carry(const ScanArgs& a, uint32_t k, uint32_t c, float (&h)[V]) {

@@ -90,3 +90,21 @@ def test_an_infinity_is_what_the_definition_makes_of_it(dt):
     assert bool(h[0, 3].isfinite()) and bool((h[1:3, 3] == inf).all()) and bool(h[3:, 3].isnan().all())
     flipped = ray_recurrence(gates, value, rays, state=state * -1)[0]
     assert bool((flipped[:, 0] == -inf).all()) and bool((flipped[:, 1] == inf).all())
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=str)
+def test_an_infinite_state_outlives_the_gates_product(dt):
+    """along 1000 rows of gates near -3, whose product over a cut's rows is below the smallest number: infinite to the end, and the gradient of an
+    infinite dlast back to the beginning"""
+    from envidr_amd.blocks import ray_recurrence
+    T, C, inf = 1000, 6, float("inf")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    gate, value = ((torch.randn(T, C, generator=g, device="cuda") * 0.5 + shift).to(dt) for shift in (-3.0, 0.0))
+    state = torch.tensor([inf, -inf] * 3, device="cuda").reshape(1, C).repeat(2, 1)
+    rays = torch.tensor([[1, 400, 600], [0, 0, 390]], dtype=torch.int32, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (gate, value, state.clone())]
+    h, last = ray_recurrence(leaves[0], leaves[1], rays, state=leaves[2])
+    owned = [*range(390), *range(400, T)]
+    assert torch.equal(last, state) and torch.equal(h[owned].float(), state[:1].expand(len(owned), C)) and not h[390:400].any()
+    dvalue, dstate = torch.autograd.grad(last, leaves[1:], -state)
+    assert torch.equal(dstate, -state) and torch.equal(dvalue[owned].float(), -state[:1].expand(len(owned), C)) and not dvalue[390:400].any()
