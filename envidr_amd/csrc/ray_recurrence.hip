@@ -563,13 +563,14 @@ template <class E, bool BACK> int run_scan(ScanArgs a, bool blend, void* workspa
     return blend ? go(std::integral_constant<int, 1>{}, std::true_type{}) : go(std::integral_constant<int, 1>{}, std::false_type{});
 }
 
+// a launch holds fewer than 2^32 threads: k_scan_map takes 64 a ray; the passes at most 64 a piece (a head of every ray, 8192 border pieces), one a
+// row and one an id
+bool scan_fits(uint64_t T, uint32_t N, uint32_t C) { return T <= 0x7FFFFFFFull && 64ull * (N + 8192ull + 8u) + T + N < 1ull << 32 && C <= (1u << 19); }
+
 int scan_checks(const char* what, uint64_t T, uint32_t N, uint32_t C, int dtype, const void* workspace, uint64_t workspace_bytes) {
     ENVIDR_REQUIRE(dtype_ok(dtype), "%s: unknown dtype %d", what, dtype);
     ENVIDR_REQUIRE(C >= 1, "%s: no channels", what);
-    // a launch holds fewer than 2^32 threads: k_scan_map takes 64 a ray; the passes at most 64 a piece (a head of every ray, 8192 border pieces),
-    // one a row and one an id
-    const uint64_t threads = 64ull * (N + 8192ull + 8u) + T + N;
-    ENVIDR_REQUIRE(T <= 0x7FFFFFFFull && threads < 1ull << 32 && C <= (1u << 19), "%s: T=%llu, N=%u or C=%u is too large", what, (unsigned long long)T, N, C);
+    ENVIDR_REQUIRE(scan_fits(T, N, C), "%s: T=%llu, N=%u or C=%u is too large", what, (unsigned long long)T, N, C);
     ENVIDR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= envidr_ray_recurrence_workspace_bytes(T, N, C) && (workspace || (T == 0 && N == 0)),
                    "%s: workspace of %llu bytes, %llu needed", what, (unsigned long long)workspace_bytes, (unsigned long long)envidr_ray_recurrence_workspace_bytes(T, N, C));
     return ENVIDR_OK;
@@ -583,11 +584,13 @@ using namespace envidr;
 extern "C" {
 
 uint64_t envidr_ray_recurrence_saved_floats(uint64_t T, uint32_t N, uint32_t C) {
+    if (!scan_fits(T, N, C)) return 0;
     const ScanPlan p = scan_plan(T, N);
     return round_up64(p.states * C, 4) + table_words(p, T, N);
 }
 
 uint64_t envidr_ray_recurrence_workspace_bytes(uint64_t T, uint32_t N, uint32_t C) {
+    if (!scan_fits(T, N, C)) return 0;
     const ScanPlan p = scan_plan(T, N);
     return 4ull * (sums_words(p, C) + table_words(p, T, N));
 }
