@@ -557,9 +557,10 @@ struct Weights {
     int64_t lg, lu, ldn;
 };
 
-// can the core read it as it is: 16-byte rows of whole units
+// can the core read it as it is: 16-byte rows of whole units, one behind the other (it bounds a tile by its rows times the pitch, which cuts rows
+// that overlap or repeat)
 bool readable(const void* p, int64_t ld, uint32_t cols, int dtype) {
-    return dtype != ENVIDR_F32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && cols % 8 == 0;
+    return dtype != ENVIDR_F32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && cols % 8 == 0 && ld >= cols;
 }
 
 struct Packer {

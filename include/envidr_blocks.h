@@ -10,7 +10,8 @@
  * envidr_last_error(), an empty batch is a successful no-op), and
  *   - `dtype` is one of ENVIDR_F32 / ENVIDR_BF16 / ENVIDR_F16 and holds for every `void*` tensor of a call; sums, activations and
  *     states are computed in 32 bits or more and rounded once where they are stored;
- *   - a row pitch (`ld*`) counts elements, the elements of a row are adjacent; the row pitch of an output is not below its width;
+ *   - a row pitch (`ld*`) counts elements, the elements of a row are adjacent; the row pitch of an output is not below its width, that of an
+ *     input may be (0: every row is the same memory);
  *   - `workspace` is caller-allocated device memory, 16-byte aligned, at least the *_workspace_bytes() of the same sizes (0 for sizes beyond
  *     an operator's limits, which the operator then refuses); it holds nothing between calls.  Two calls that may run at the same time (two streams, two captured graphs) need a workspace each;
  *   - an output overlaps no input and no other output, except where it is said to.
