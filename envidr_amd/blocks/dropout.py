@@ -56,13 +56,18 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Tensor
 
 class CounterDropout(torch.nn.Module):
     """`dropout` with a generator of its own: in training every forward call takes the next call number (on the device, so a captured step draws
-    a new mask at every replay); in evaluation x (+ residual) passes through.  One instance belongs to one stream at a time."""
+    a new mask at every replay); in evaluation x (+ residual) passes through.  One instance belongs to one stream at a time.
 
-    def __init__(self, p: float = 0.1, seed: int = 0):
+    seed: the generator's key.  Modules of one key that are called in step drop the same elements; without a seed the key is drawn from torch's
+    default CPU generator, another for each module and the same again after `torch.manual_seed`."""
+
+    def __init__(self, p: float = 0.1, seed: int | None = None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise _lib.EnvidrError(f"CounterDropout: p={p} is not a probability")
         self.p = float(p)
+        if seed is None:
+            seed = int(torch.empty((), dtype=torch.int64, device="cpu").random_())
         self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:

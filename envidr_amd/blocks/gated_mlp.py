@@ -95,9 +95,9 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
 class GatedMLP(torch.nn.Module):
     """A gated feed-forward block of width d_in -> d_hidden -> d_out (d_in when not given), without biases.  residual: adds x to the result; p: dropout
-    on the result in training."""
+    on the result in training, its masks from `seed` (`CounterDropout`'s)."""
 
-    def __init__(self, d_in: int, d_hidden: int, d_out: int | None = None, activation: str = "silu", residual: bool = False, p: float = 0.0, seed: int = 0):
+    def __init__(self, d_in: int, d_hidden: int, d_out: int | None = None, activation: str = "silu", residual: bool = False, p: float = 0.0, seed: int | None = None):
         super().__init__()
         d_out = d_in if d_out is None else d_out
         if residual and d_out != d_in:
