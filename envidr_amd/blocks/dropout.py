@@ -59,7 +59,11 @@ class CounterDropout(torch.nn.Module):
     a new mask at every replay); in evaluation x (+ residual) passes through.  One instance belongs to one stream at a time.
 
     seed: the generator's key.  Modules of one key that are called in step drop the same elements; without a seed the key is drawn from torch's
-    default CPU generator, another for each module and the same again after `torch.manual_seed`."""
+    default CPU generator, another for each module and the same again after `torch.manual_seed`.
+
+    A pass that is run twice (activation checkpoints) has to draw twice alike: take the call's generator first, rng = module.draw(), and hand it to
+    the forward call that is checkpointed, checkpoint(module, x, rng=rng).  A training call without one inside a backward pass is refused: its mask
+    would not be the one of the pass that it repeats."""
 
     def __init__(self, p: float = 0.1, seed: int | None = None):
         super().__init__()
@@ -70,16 +74,28 @@ class CounterDropout(torch.nn.Module):
             seed = int(torch.empty((), dtype=torch.int64, device="cpu").random_())
         self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
 
-    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+    def draw(self) -> torch.Tensor:
+        """the generator's next call: a copy of its own, for `forward` and for `dropout`"""
+        if not self.rng.is_cuda:
+            raise _lib.EnvidrError(f"CounterDropout: the generator is on {self.rng.device}: move the module to the GPU")
+        used = torch.empty_like(self.rng)
+        with _bind.on_device(self.rng) as stream:
+            _bind.check(_bind.lib().envidr_dropout_step(self.rng.data_ptr(), used.data_ptr(), stream), "envidr_dropout_step")
+        return used
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, rng: torch.Tensor | None = None) -> torch.Tensor:
         if not self.training or self.p == 0.0:
             return x if residual is None else x + residual
         _bind.same_kind("CounterDropout", x, residual=residual)
-        if self.rng.device != x.device:
-            raise _lib.EnvidrError(f"CounterDropout: the generator is on {self.rng.device}, x on {x.device}: move the module")
-        used = torch.empty_like(self.rng)
-        with _bind.on_device(x) as stream:
-            _bind.check(_bind.lib().envidr_dropout_step(self.rng.data_ptr(), used.data_ptr(), stream), "envidr_dropout_step")
-        return dropout(x, self.p, used, residual=residual)
+        if rng is None:
+            if self.rng.device != x.device:
+                raise _lib.EnvidrError(f"CounterDropout: the generator is on {self.rng.device}, x on {x.device}: move the module")
+            # (the number of the backward pass that this thread is in: what torch's own checkpoints go by)
+            if torch._C._current_graph_task_id() != -1:
+                raise _lib.EnvidrError("CounterDropout: called inside a backward pass, where a recomputed call would draw another mask: give it the "
+                                       "first call's generator (rng = module.draw(), module(x, rng=rng))")
+            rng = self.draw()
+        return dropout(x, self.p, rng, residual=residual)
 
     def extra_repr(self) -> str:
         return f"p={self.p}"

@@ -112,6 +112,7 @@ class GatedMLP(torch.nn.Module):
             torch.nn.init.xavier_uniform_(w)
         self.drop = CounterDropout(p, seed)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
+        """rng: the dropout's call (`self.drop.draw()`), for a pass that is run twice"""
         y = gated_mlp(x, self.w_gate, self.w_up, self.w_down, self.activation)
-        return self.drop(y, residual=x if self.residual else None)
+        return self.drop(y, residual=x if self.residual else None, rng=rng)

@@ -1,6 +1,7 @@
-"""Where CounterDropout's masks come from: a key of its own for every module."""
+"""Where CounterDropout's masks come from: a key of its own for every module, a call's own copy of the generator for what is computed twice."""
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 
 def test_modules_have_keys_of_their_own():
@@ -23,3 +24,68 @@ def test_modules_draw_masks_of_their_own():
     x = torch.ones(4096, device="cuda")
     same = float((a(x) == b(x)).float().mean())
     assert 0.4 < same < 0.6                                       # (independent halves agree at half the places: 4096 of them, a deviation of 1/128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_a_recomputed_pass_draws_the_same_mask_or_none(reentrant):
+    """activation checkpoints run the forward pass again inside the backward one: with the call's own generator the gradient is the plain pass's;
+    without it the module refuses to draw another mask"""
+    from envidr_amd._lib import EnvidrError
+    from envidr_amd.blocks import CounterDropout, GatedMLP
+    torch.manual_seed(3)
+    drop, block = CounterDropout(0.5, seed=1).cuda().train(), GatedMLP(24, 64, residual=True, p=0.5).cuda().train()
+    for module, own in ((drop, drop), (block, block.drop)):
+        x = torch.randn(300, 24, device="cuda", requires_grad=True)
+        dy = torch.randn(300, 24, device="cuda")
+        before = int(own.rng[1])
+        rng = own.draw()
+        assert rng.tolist() == [int(own.rng[0]), before] and int(own.rng[1]) == before + 1
+        plain = module(x, rng=rng)
+        again = checkpoint(module, x, rng=rng, use_reentrant=False) if not reentrant else checkpoint(lambda t: module(t, rng=rng), x, use_reentrant=True)
+        assert torch.equal(plain, again) and int(own.rng[1]) == before + 1
+        wanted = [x, *(p for p in module.parameters())]
+        first = torch.autograd.grad(plain, wanted, dy)
+        if reentrant:                                             # (torch.autograd.grad is not for this kind)
+            x.grad = None
+            module.zero_grad()
+            again.backward(dy)
+            second = [t.grad for t in wanted]
+        else:
+            second = torch.autograd.grad(again, wanted, dy)
+        assert all(torch.equal(p, q) for p, q in zip(first, second))
+        y = checkpoint(module, x, use_reentrant=reentrant)
+        calls = int(own.rng[1])
+        with pytest.raises(EnvidrError, match="inside a backward pass"):
+            y.backward(dy)
+        assert int(own.rng[1]) == calls
+        module.eval()
+        checkpoint(module, x, use_reentrant=reentrant).backward(dy)       # (nothing is drawn in evaluation)
+        module.train()
+
+
+@pytest.mark.gpu
+def test_a_call_with_its_own_generator_is_checked():
+    from envidr_amd._lib import EnvidrError
+    from envidr_amd.blocks import CounterDropout
+    drop = CounterDropout(0.5, seed=1).cuda().train()
+    x = torch.ones(64, device="cuda")
+    for bad in (torch.zeros(2, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda"), torch.zeros(2, dtype=torch.int64)):
+        with pytest.raises(EnvidrError, match="int64"):
+            drop(x, rng=bad)
+    assert drop.rng.tolist() == [1, 0]
+
+
+@pytest.mark.gpu
+def test_recomputation_never_gives_the_gradient_of_another_mask():
+    """a checkpointed call without a generator of its own: an error, or the gradient of the mask that was drawn"""
+    from envidr_amd._lib import EnvidrError
+    from envidr_amd.blocks import CounterDropout
+    drop = CounterDropout(0.5, seed=1).cuda().train()
+    x = torch.ones(5000, device="cuda", requires_grad=True)
+    y = checkpoint(drop, x, use_reentrant=False)
+    try:
+        y.sum().backward()
+    except EnvidrError:
+        return
+    assert torch.equal(x.grad, y.detach())
