@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -57,6 +58,19 @@ def same_kind(name: str, first: torch.Tensor, **others: torch.Tensor | None) -> 
         if t is not None and (t.dtype != dtype or t.device != device):
             raise _lib.EnvidrError(f"{name}: {what} is {t.dtype} on {t.device}, the first tensor {dtype} on {device}")
     return DTYPES[dtype]
+
+
+def differentiated(*tensors: torch.Tensor | None) -> bool:
+    """must a call on these go through its autograd function: for their gradients, or, where forward-mode derivatives are being taken (a tensor
+    that carries a tangent requires no gradient), for torch's refusal there"""
+    if forward_ad._current_level >= 0:
+        return True
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def sizes(name: str, **n: int) -> None:

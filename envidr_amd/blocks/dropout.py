@@ -49,7 +49,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Tensor
             raise _lib.EnvidrError(f"dropout: residual {tuple(residual.shape)} is not x {tuple(x.shape)}")
         residual = residual.contiguous()
     x = x.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
+    if _bind.differentiated(x, residual):
         return _Dropout.apply(x, residual, rng, p, code)
     return _launch(x, residual, rng, p, code)
 

@@ -86,7 +86,7 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if 0 in w_gate.shape or 0 in w_down.shape:
         raise _lib.EnvidrError("gated_mlp: a width is zero")
     rows = _rows(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+    if _bind.differentiated(x, w_gate, w_up, w_down):
         y = _GatedMlp.apply(rows, _rows(w_gate), _rows(w_up), _rows(w_down), code, ACTIVATIONS[activation])
     else:
         y = _forward(rows, _rows(w_gate), _rows(w_up), _rows(w_down), code, ACTIVATIONS[activation])

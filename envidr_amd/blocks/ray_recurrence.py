@@ -81,7 +81,7 @@ def ray_recurrence(gate: torch.Tensor, value: torch.Tensor, rays: torch.Tensor, 
         raise _lib.EnvidrError(f"ray_recurrence: state is float32 [{rays.shape[0]}, {gate.shape[1]}] on {gate.device}, not {state.dtype} {tuple(state.shape)} on {state.device}")
     gate, value, rays = gate.contiguous(), value.contiguous(), rays.contiguous()
     state = None if state is None else state.contiguous()
-    if torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or state is not None and state.requires_grad):
+    if _bind.differentiated(gate, value, state):
         return _RayRecurrence.apply(gate, value, state, rays, code, int(blend))
     h, last, _ = _forward(gate, value, rays, state, code, int(blend), False)
     return h, last
