@@ -38,13 +38,24 @@ struct PackJob {
 struct PackJobs {
     PackJob job[5];
     uint32_t n;
+    uint32_t from;                  // the launch's first block
 };
 
+// Grids that grow with the data are launched in runs: a launch holds fewer than 2^32 threads.  (Blocks that walk instead cost the sums of a
+// training pass of 4096 rows, 512 -> 2048 -> 512 in bf16, 14 us for 12.)
+constexpr uint32_t kMostBlocks = (1u << 31) / kBlock;
+template <class Launch> int in_runs(uint32_t blocks, Launch launch) {
+    for (uint32_t from = 0; from < blocks; from += kMostBlocks)
+        if (int rc = launch(from, blocks - from < kMostBlocks ? blocks - from : kMostBlocks)) return rc;
+    return ENVIDR_OK;
+}
+
 template <class E, class T, int NP> __global__ void __launch_bounds__(kBlock) k_pack_operands(PackJobs a) {
+    const uint32_t block = a.from + blockIdx.x;
     uint32_t j = 0;
-    while (j + 1 < a.n && blockIdx.x >= a.job[j + 1].first_block) ++j;
+    while (j + 1 < a.n && block >= a.job[j + 1].first_block) ++j;
     const PackJob p = a.job[j];
-    const uint64_t at = (uint64_t)(blockIdx.x - p.first_block) * kBlock + threadIdx.x;
+    const uint64_t at = (uint64_t)(block - p.first_block) * kBlock + threadIdx.x;
     const uint64_t row = at / p.units;
     if (row >= p.rows) return;
     const uint32_t c0 = (uint32_t)(at % p.units) * 8u;
@@ -293,14 +304,16 @@ struct SumJob {
 struct SumArgs {
     SumJob job[3];
     uint32_t jobs, splits;
+    uint32_t from;                  // the launch's first block
 };
 // SHARE threads add up a result's parts, every SHARE-th each, and the first adds theirs
 template <class E, int SHARE> __global__ void __launch_bounds__(kBlock) k_sum_splits(SumArgs a) {
     constexpr uint32_t kResults = kBlock / SHARE;
+    const uint32_t block = a.from + blockIdx.x;
     uint32_t j = 0;
-    while (j + 1 < a.jobs && blockIdx.x >= a.job[j + 1].first_block) ++j;
+    while (j + 1 < a.jobs && block >= a.job[j + 1].first_block) ++j;
     const SumJob& s = a.job[j];
-    const uint64_t i = (uint64_t)(blockIdx.x - s.first_block) * kResults + threadIdx.x % kResults;
+    const uint64_t i = (uint64_t)(block - s.first_block) * kResults + threadIdx.x % kResults;
     float v = 0;
     if (i < s.n) {
 #pragma unroll 8
@@ -595,9 +608,11 @@ struct Packer {
         return o;
     }
     template <class E, class T, int NP> int launch(hipStream_t s) {
-        if (jobs.n == 0) return ENVIDR_OK;
-        hipLaunchKernelGGL((k_pack_operands<E, T, NP>), dim3(blocks), dim3(kBlock), 0, s, jobs);
-        return check_launch("k_pack_operands");
+        return in_runs(blocks, [&](uint32_t from, uint32_t n) {
+            jobs.from = from;
+            hipLaunchKernelGGL((k_pack_operands<E, T, NP>), dim3(n), dim3(kBlock), 0, s, jobs);
+            return check_launch("k_pack_operands");
+        });
     }
 };
 
@@ -636,9 +651,12 @@ struct Sums {
         blocks += (uint32_t)((n + results - 1) / results);
     }
     template <class E> int launch(hipStream_t s) {
-        if (share == 4u) hipLaunchKernelGGL((k_sum_splits<E, 4>), dim3(blocks), dim3(kBlock), 0, s, a);
-        else hipLaunchKernelGGL((k_sum_splits<E, 1>), dim3(blocks), dim3(kBlock), 0, s, a);
-        return check_launch("k_sum_splits");
+        return in_runs(blocks, [&](uint32_t from, uint32_t n) {
+            a.from = from;
+            if (share == 4u) hipLaunchKernelGGL((k_sum_splits<E, 4>), dim3(n), dim3(kBlock), 0, s, a);
+            else hipLaunchKernelGGL((k_sum_splits<E, 1>), dim3(n), dim3(kBlock), 0, s, a);
+            return check_launch("k_sum_splits");
+        });
     }
 };
 // the weights' gradients from their parts, which lie one behind the other
