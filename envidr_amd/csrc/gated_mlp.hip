@@ -87,6 +87,20 @@ struct GluArgs {
     uint32_t col_tiles, tiles;
 };
 
+// The units that fill the last operand unit up (columns F .. Fp - 1) have weights of zero, which an infinity in x or dy makes NaN: they are cleared, or
+// the next product would carry that into its whole row.  (fp32 operands with an infinity are NaN anyway.)
+template <int NP, int B, int N> __device__ __forceinline__ void clear_behind(float (&v)[B][N][4], uint32_t f0, uint32_t F) {
+    if (NP == 3 || f0 + N * 16u <= F) return;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool behind = f0 + j * 16u + 4u * (threadIdx.x >> 4 & 3u) + r >= F;
+#pragma unroll
+            for (int b = 0; b < B; ++b) v[b][j][r] = behind ? 0.0f : v[b][j][r];
+        }
+}
+
 template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ void __launch_bounds__(WM* WN * 64, 2) k_glu_forward(GluArgs a) {
     using P = Product<T, NP, TM, 2 * TF, WM, WN, true, true, true>;
     using Out = PlaneStore<T, NP, P::NI * 8>;
@@ -118,6 +132,7 @@ template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ v
                     for (int r = 0; r < 4; ++r) {
                         h[b][j][r] = activation_value<ACT, NP == 3>(acc[mi + b][2 * j][r]) * acc[mi + b][2 * j + 1][r];
                     }
+            clear_behind<NP>(h, f0, a.F);
             Out::store(scratch, h, a.h, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
         }
     }
@@ -162,6 +177,8 @@ template <class T, int NP, int TM, int TF, int WM, int WN, int ACT> __global__ v
                         dg[b][j][r] = d * u * slope;
                         du[b][j][r] = d * act;
                     }
+            clear_behind<NP>(dg, f0, a.F);
+            clear_behind<NP>(du, f0, a.F);
             Out::store(scratch, h, a.h, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
             Out::store(scratch, dg, a.dg, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);
             Out::store(scratch, du, a.du, a.plane, a.Fp, a.M, row0 + mi * 16u, f0, a.Fp);

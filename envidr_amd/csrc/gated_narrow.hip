@@ -100,6 +100,12 @@ template <class E, int ACT, int KD, int OB> __global__ void __launch_bounds__(na
                     for (int q = 0; q < 4; ++q) {
                         v.v[4 * b + q] = from_f32<E>(activation_value<ACT, false>(p[mi][b][q]) * p[mi][b + 2][q]);
                     }
+                // (units behind the last one: weights of zero, which an infinity in x makes NaN)
+                if (hb * 32u + 32u > a.F) {
+#pragma unroll
+                    for (int n = 0; n < 8; ++n)
+                        if (hb * 32u + 16u * (n >> 2) + 4u * g + (n & 3) >= a.F) v.v[n] = from_f32<E>(0.0f);
+                }
                 h[mi] = __builtin_bit_cast(s16x8, v);
             }
 #pragma unroll

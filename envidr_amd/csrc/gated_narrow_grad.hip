@@ -33,6 +33,18 @@ __device__ __forceinline__ s16x8 columns(uint32_t at, uint32_t pitch, uint32_t l
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Units behind the last one have weights of zero, which an infinity in x or dy makes NaN, and dx takes all units of a team: they are cleared.  All ones
+// for those of a lane's eight units that are there.  (From a lane number that the compiler takes for a new one: what it kept of this across the
+// loop over the rows would be spilled.)
+__device__ __forceinline__ s16x8 present_units(uint32_t lane, uint32_t first, uint32_t F) {
+    asm volatile("" : "+v"(lane));
+    const uint32_t f = first + 4u * (lane >> 4);
+    s16x8 keep;
+#pragma unroll
+    for (uint32_t n = 0; n < 8; ++n) keep[n] = f + 16u * (n >> 2) + (n & 3u) < F ? -1 : 0;
+    return keep;
+}
+
 // DB: blocks of 16 input columns; ONE: one team, whose rows are one 16-byte unit a thread at most
 template <class E, int ACT, int DB, bool ONE> __global__ void __launch_bounds__(kWaves * 64, 2) k_narrow_backward(NarrowGradArgs a) {
     constexpr int KD = (DB + 1) / 2;                                             // k blocks of 32 of them
@@ -41,6 +53,7 @@ template <class E, int ACT, int DB, bool ONE> __global__ void __launch_bounds__(
     __shared__ __attribute__((aligned(1024))) char lds_all[kLds];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15u;
     const uint32_t slices = ONE ? kWaves : a.slices, team = ONE ? 0u : wave / slices, slice = ONE ? wave : wave % slices, teams = kWaves / slices, blocks = (a.D + 15u) / 16u;
+    const uint32_t used = ONE ? (a.F + 63u) / 64u * 2u : (a.F + 31u) / 32u;         // blocks of 32 units that dx is formed of (ONE: in pairs)
     const uint32_t h_pitch = slices * 64u + 32u, hidden = slices * 32u;
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)lds_all, lds_w = lds, team_bytes = kTeamRows * (kXPitch + kDyPitch + 2u * h_pitch), teams_at = lds + 2u * hidden * kXPitch;
     const uint32_t xs = teams_at + team * team_bytes, ys = xs + kTeamRows * kXPitch, dgs = ys + kTeamRows * kDyPitch, dus = dgs + kTeamRows * h_pitch;
@@ -116,7 +129,8 @@ template <class E, int ACT, int DB, bool ONE> __global__ void __launch_bounds__(
     for (;;) {
         const bool more = t + gridDim.x < tiles;
         if (more) fetch(t + gridDim.x);
-        Pack<E, 8> vh[2], vg[2], vu[2];
+        using Units8 = Pack<E, 8>;
+        Units8 vh[2], vg[2], vu[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             f32x4 pg[2] = {}, pu[2] = {}, dh[2];
@@ -143,6 +157,16 @@ template <class E, int ACT, int DB, bool ONE> __global__ void __launch_bounds__(
                     vg[rb].v[4 * b + q] = from_f32<E>(dh[rb][q] * pu[rb][q] * slope);
                     vu[rb].v[4 * b + q] = from_f32<E>(dh[rb][q] * act);
                 }
+        }
+        if constexpr (!ONE) {
+            if (slice * 32u + 32u > a.F) {
+                const s16x8 keep = present_units(lane, slice * 32u, a.F);
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb) {
+                    vg[rb] = __builtin_bit_cast(Units8, (s16x8)(__builtin_bit_cast(s16x8, vg[rb]) & keep));
+                    vu[rb] = __builtin_bit_cast(Units8, (s16x8)(__builtin_bit_cast(s16x8, vu[rb]) & keep));
+                }
+            }
         }
         s16x8 du[2];
 #pragma unroll
@@ -188,6 +212,20 @@ template <class E, int ACT, int DB, bool ONE> __global__ void __launch_bounds__(
                 }
             }
         }
+        if constexpr (ONE) {                 // (here, where nothing but the sums is in registers, as these are short)
+            if (slice * 32u + 32u > a.F && slice < used) {
+                const s16x8 keep = present_units(lane, slice * 32u, a.F);
+                uint32_t l = lane;
+                asm volatile("" : "+v"(l));
+                const uint32_t at = (l & 15u) * h_pitch + (slice * 4u + (l >> 4)) * 16u;
+#pragma unroll
+                for (uint32_t rb = 0; rb < 2; ++rb) {
+                    lds_s16x8 *pg = (lds_s16x8*)(dgs + at + rb * 16u * h_pitch), *pu = (lds_s16x8*)(dus + at + rb * 16u * h_pitch);
+                    *pg &= keep;
+                    *pu &= keep;
+                }
+            }
+        }
         lds_barrier();
         if (a.dx) {
 #pragma unroll 1
@@ -216,15 +254,15 @@ template <class E, int ACT, int DB, bool ONE> __global__ void __launch_bounds__(
                 if constexpr (ONE) {
                     read(now, 0);
 #pragma unroll 1
-                    for (uint32_t hb = 0; hb < slices; hb += 2) {
+                    for (uint32_t hb = 0; hb < used; hb += 2) {
                         read(next, hb + 1);
                         multiply(now);
-                        if (hb + 2 < slices) read(now, hb + 2);
+                        if (hb + 2 < used) read(now, hb + 2);
                         multiply(next);
                     }
                 } else {                     // (two sets of operands and several teams' rows would not fit the registers)
 #pragma unroll 1
-                    for (uint32_t hb = 0; hb < slices; ++hb) {
+                    for (uint32_t hb = 0; hb < used; ++hb) {
                         read(now, hb);
                         multiply(now);
                     }
