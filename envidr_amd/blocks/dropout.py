@@ -58,8 +58,8 @@ class CounterDropout(torch.nn.Module):
     """`dropout` with a generator of its own: in training every forward call takes the next call number (on the device, so a captured step draws
     a new mask at every replay); in evaluation x (+ residual) passes through.  One instance belongs to one stream at a time.
 
-    seed: the generator's key.  Modules of one key that are called in step drop the same elements; without a seed the key is drawn from torch's
-    default CPU generator, another for each module and the same again after `torch.manual_seed`.
+    seed: the generator's key.  Modules of one key that are called in step drop the same elements (so do a module and its copy); without a seed the key
+    is drawn from torch's default CPU generator, another for each module and the same again after `torch.manual_seed`.
 
     A pass that is run twice (activation checkpoints) has to draw twice alike: take the call's generator first, rng = module.draw(), and hand it to
     the forward call that is checkpointed, checkpoint(module, x, rng=rng).  A training call without one inside a backward pass is refused: its mask

@@ -76,7 +76,9 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     One dtype (float32, bfloat16 or float16) and one device for all; any strides; activation "silu", "gelu" (tanh form), "relu" or
     "sigmoid".  Differentiable once, w.r.t. every tensor.  Products accumulate in 32 bits; in the 16-bit dtypes the hidden layer is rounded
-    to the dtype once, between the products.  float32 carries 24-bit operands through the bf16 matrix cores; an infinity in them gives NaN."""
+    to the dtype once, between the products (forward of up to 32 rows: not at all).  float32 carries 24-bit operands through the bf16 matrix cores
+    (beyond 64 rows: an infinity in them gives NaN, and of numbers below 2^-108 what is above 2^-126 counts).  torch.autocast casts nothing here: inside
+    such a region the caller gives x and the weights one dtype.  A forward-mode tangent is refused."""
     code = _bind.same_kind("gated_mlp", x, w_gate=w_gate, w_up=w_up, w_down=w_down)
     if activation not in ACTIVATIONS:
         raise _lib.EnvidrError(f"gated_mlp: activation {activation!r} is not one of {', '.join(ACTIVATIONS)}")

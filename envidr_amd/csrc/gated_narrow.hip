@@ -6,7 +6,7 @@
 //   a lane holds h of units 4 g' .. 4 g' + 3 of both blocks (g' = lane / 16) for its row: exactly eight k of the next product's operand, in an
 //   order of k that Wd's rows in LDS follow, so y += h Wd^T needs no exchange between lanes.
 // Bound: the activation on the vector ALU (two quarter-rate instructions and about eight others a hidden unit and row), then the products.
-// 524 288 rows of 72 -> 256 -> 12 in fp16: 74 us; 99 991 rows 22 us (in two kernels, h through memory: 70).
+// 524 288 rows of 72 -> 256 -> 12 in fp16: 78 us; 99 991 rows 22 us (in two kernels, h through memory: 70).
 #include "gated_mlp.hip.h"
 #include "gemm_core.hip.h"
 

@@ -7,8 +7,8 @@
 // that the lanes' parts of Wd follow.  So a wave forms its units' share of y by itself; the shares meet in LDS and are added up in the order of the
 // units.
 // Bound: matrix cores (six products a product: about 45 % of the time) and vector ALU (activation, terms of h: 40 %), which the two waves of a SIMD
-// use in turns.  146 000 rows of 72 -> 256 -> 12: 100 us (operands laid out and the hidden layer through memory: 232); of 32 -> 64 -> 16 31 (71);
-// 65 rows 18 (30).
+// use in turns.  146 000 rows of 72 -> 256 -> 12: 104 us by itself, 119 behind a backward pass, whose operands have taken x's place in the caches (operands
+// laid out and the hidden layer through memory: 232); of 32 -> 64 -> 16 30 (71); 65 rows 18 (30).
 #include "gated_mlp.hip.h"
 #include "gemm_core.hip.h"
 

@@ -343,8 +343,8 @@ template <class E, int ACT> int launch(const NarrowGradArgs& a, uint32_t grid, h
 
 }  // namespace
 
-// Widths whose gradients' sums fit eight waves' registers.  Against the tiles, a training pass in bf16: 146 000 rows of 72 -> 256 -> 12 245 -> 131 us, of 96 -> 33
-// -> 32 141 -> 111, of 32 -> 64 -> 16 126 -> 45; 10 000 rows of 72 -> 256 -> 12 51 both; 65 rows 35 -> 32.
+// Widths whose gradients' sums fit eight waves' registers.  Against the tiles, a training pass in bf16: 146 000 rows of 72 -> 256 -> 12 245 -> 130 us, of 96 -> 33
+// -> 32 141 -> 108, of 32 -> 64 -> 16 126 -> 45; 10 000 rows of 72 -> 256 -> 12 51 both; 65 rows 35 -> 32.
 bool gated_grad_is_narrow(uint32_t D, uint32_t F, uint32_t O, int dtype) { return dtype != ENVIDR_F32 && D <= 96 && F <= 256 && O <= 32; }
 
 uint32_t gated_narrow_grad_parts(uint32_t M, uint32_t D, uint32_t F) {

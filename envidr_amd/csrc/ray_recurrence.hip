@@ -14,10 +14,11 @@
 //   k_scan_join, k_scan_carry   the maps in order -> the state at every border
 //   k_scan_forward / k_scan_backward   per piece: rows in blocks of kRows, the next block loaded under the present one; rows that neither a
 //                  mark nor an owner claims get zeros, and ids that no ray names keep their state
-// Short rays are one piece each and pay for none of the middle; cut rays are read twice by k_scan_sums.  With at most a row a ray or few
-// rows in all nothing is cut: two launches instead of five.
+// A ray that no border falls into is one piece and pays for none of the middle; of a cut one, whatever its length, the rows between a border and the
+// next are read a second time by k_scan_sums (4096 rays of 36 rows on average: 43 % of the rays, half the rows).  With at most a row a ray or few rows
+// in all nothing is cut: two launches instead of five.
 // Lanes are channels, two each in the 16-bit types where C is even (a row of 128 channels is then one 256-byte access of a wave, not two of 128:
-// 222 us a training pass of three sequences, 300 k rows, bf16; 226 with one channel a lane).  From 64 lanes a row on a wave has one piece, and rows,
+// 230 us a training pass of three sequences, 300 k rows, bf16; 233 with one channel a lane).  From 64 lanes a row on a wave has one piece, and rows,
 // bounds and addresses live on the scalar unit; with fewer channels 64 / lanes pieces share a wave.
 // The backward pass needs h_{t-1}.  It does not read the stored (rounded) h: the forward pass leaves the 32-bit state at every kRows-th row
 // (`saved`), and a block's states are formed again from there in registers.
@@ -39,8 +40,10 @@ struct ScanPlan {
 
 ScanPlan scan_plan(uint64_t T, uint32_t N) {
     ScanPlan p{};
-    // Not cut: at most 256 rows (46 us a training pass against 56 cut; at 512 rows 82 against 57), or at most a row a ray -- the step of many
-    // rays with their states (1000 rows of 256 channels forward: 31 against 41 us).  Anything else may hide a ray that is nearly all of T.
+    // Not cut: at most 256 rows (46 us a training pass against 56 cut; at 512 rows 82 against 57), or at most a row a ray on average -- the step of
+    // many rays with their states (1000 rays of one row, 64 channels: 16 us a training pass against 30 cut).  The price of the second: where most
+    // rays are empty, a long one among them is walked by one wave (4096 rows in four rays, training: rays of 300 rows 90 us against 64 cut, of
+    // 1000 rows 277 against 65).  Anything else may hide a ray that is nearly all of T.
     if (T > 256 && T > N) {
         // 64 rows, doubled until at most 8192 borders (128 segments) are left.  (Three sequences, 300 k rows of 128 channels in bf16: with
         // pieces of 256 rows and blocks of 16 a wave a SIMD is left to its own latencies -- sums 47, forward 51, backward 125 us; 34, 44, 73 so.)

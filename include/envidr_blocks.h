@@ -38,8 +38,8 @@ int envidr_blocks_abi_version(void);
  *   x [M, D], Wg / Wu [F, D], Wd [O, F], y [M, O].  D, F, O >= 1 of any remainder; 16-bit types: fastest where widths and pitches are
  *   multiples of 8 and the tensors 16-byte aligned.
  * Arithmetic.  16-bit types: products on the 16-bit matrix cores, accumulated in fp32; h (forward) and dg, du, h (backward) are rounded
- * to the type once, as the next product's operands.  fp32: every operand is carried as three bf16 terms (24 significant bits), the six
- * products above 2^-24 are accumulated in fp32; an infinity in an operand gives NaN.  Up to 32 rows (fp32: 64) go forward through a
+ * to the type once, as the next product's operands.  fp32: every operand is carried as three bf16 terms (24 significant bits; of
+ * numbers below 2^-108 what is above 2^-126), the six products above 2^-24 are accumulated in fp32; an infinity in an operand gives NaN.  Up to 32 rows (fp32: 64) go forward through a
  * kernel that streams the weights once (fp32: on the fp32 matrix cores) and keeps h in 32 bits.  fp16: a hidden unit above 65504 is an infinity.
  * Limits: D, F, O <= 2^20, F D and O F <= 2^32, M < 2^31 - 256, row pitches <= 2^21.
  * backward: dx [M, D], dw_gate / dw_up [F, D], dw_down [O, F] (any of them may be NULL: not computed).  It needs x, dy and the weights
@@ -62,7 +62,8 @@ int envidr_gated_mlp_backward(const void* dy, int64_t lddy, const void* x, int64
  *   row or an id.  A ray with count <= 0, offset < 0 or offset + count > T has no rows (the compositors' rule).
  *   state fp32 [N, C] or NULL (zeros): h before the first sample, indexed by id; last fp32 [N, C]: h after the last one.  The id of a ray
  *   without rows, and an id that no ray names, keep their state; a ray with an id outside 0 .. N-1 starts from zeros and leaves none.
- *   Rows that belong to no ray: h, dgate and dvalue are zero there.  A NaN or an infinity stays with its ray and channel, and along them.
+ *   Rows that belong to no ray: h, dgate and dvalue are zero there.  A NaN or an infinity stays with its ray and channel, and along them
+ *   (an infinity is one, or NaN from a row on whose gate is below -87: its weight is 0 in 32 bits).
  *   Limits: T < 2^31, 65 N + T < 2^32 - 2^20, C <= 2^19.
  *   saved: fp32 [envidr_ray_recurrence_saved_floats(T, N, C)] or NULL; written by the forward pass and read by the backward one of the
  *   same inputs.
