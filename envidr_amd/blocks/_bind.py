@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd import forward_ad
@@ -71,6 +72,22 @@ def differentiated(*tensors: torch.Tensor | None) -> bool:
         if t is not None and t.requires_grad:
             return True
     return False
+
+
+def differentiable_once(backward):
+    """for the `backward` of an autograd function: under create_graph its gradients, differentiated again, raise.  (torch's own decorator asks the
+    incoming gradient only: where that is a constant, as for normals by autograd.grad(sdf, positions, ones, create_graph=True), it hands out constants,
+    and a loss on them would silently lose its gradient.)"""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        out = out if isinstance(out, tuple) else (out,)
+        error = torch._C._functions.DelayedError(b"the block operators are differentiable once: their gradients have none", len(out))
+        return error(*(None if t is None else t.detach().requires_grad_(True) for t in out))
+    return run
 
 
 def sizes(name: str, **n: int) -> None:

@@ -25,7 +25,7 @@ class _Dropout(torch.autograd.Function):
         return _launch(x, residual, rng, p, code)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_bind.differentiable_once
     def backward(ctx, dy):
         (rng,) = ctx.saved_tensors
         dx = _launch(dy.contiguous(), None, rng, ctx.p, ctx.code) if ctx.needs_input_grad[0] else None

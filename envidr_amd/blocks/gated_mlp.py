@@ -54,7 +54,7 @@ class _GatedMlp(torch.autograd.Function):
         return _forward(x, wg, wu, wd, code, act)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_bind.differentiable_once
     def backward(ctx, dy):
         x, wg, wu, wd = ctx.saved_tensors
         lib = _bind.lib()

@@ -43,7 +43,7 @@ class _RayRecurrence(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_bind.differentiable_once
     def backward(ctx, dh, dlast):
         gate, value, state, rays, saved = ctx.saved_tensors
         lib = _bind.lib()
